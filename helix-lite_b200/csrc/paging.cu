@@ -1,0 +1,393 @@
+// Block tables and slot maps of a batch, built on the GPU from its requests'
+// lengths, and the way back: pages given up when sequences shrink or end.
+//
+// With page size S, c_b tokens cached and n_b new ones, sequence b holds
+// have_b = ceil(c_b / S) pages and needs need_b = ceil((c_b + n_b) / S). The
+// call's new pages are numbered k sequence by sequence; page k is
+// free[count - 1 - k] (the free list is a stack). Token i of the packed batch
+// belongs to the sequence whose query_start interval holds i; its position is
+// c_b + i - query_start[b] and its slot page * S + position % S.
+//
+// Both kernels are bound by launch latency except for large prompts, where
+// extend writes 16 bytes a token. So every CTA of extend repeats the scan over
+// the batch (B lengths from L2; no message between CTAs, one launch) and then
+// writes its own stretch of tokens and pages; page k comes straight from the
+// free stack, never from a table entry that another CTA writes. Truncate runs
+// as one CTA, since reference counts of shared pages need block-wide steps.
+#include "common.cuh"
+
+namespace hx {
+namespace pg {
+
+constexpr int NT = 512;          // threads of a CTA of extend
+constexpr int NTT = 1024;        // threads of truncate's CTA
+constexpr int MAXB = 16384;      // sequences a call takes (their prefix sums sit in shared memory)
+constexpr int kTokensPerCta = 2048;
+
+// Inclusive scan of (a, b) over the block's threads; totals to every thread.
+template <int N>
+HX_DEVINL void block_scan2(long long& a, long long& b, long long& ta, long long& tb, long long (*ws)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += x, b += y;
+  }
+  if (lane == 31) ws[warp][0] = a, ws[warp][1] = b;
+  __syncthreads();
+  long long pa = 0, pb = 0;
+  ta = tb = 0;
+#pragma unroll 4
+  for (int w = 0; w < N / 32; ++w) {
+    if (w < warp) pa += ws[w][0], pb += ws[w][1];
+    ta += ws[w][0], tb += ws[w][1];
+  }
+  a += pa;
+  b += pb;
+  __syncthreads();
+}
+
+// Largest b with first[b] <= i (first ascending, first[0] = 0): the sequence
+// holding item i; sequences without items are passed over.
+HX_DEVINL int find_row(const int* first, int B, int i) {
+  int lo = 0, hi = B;  // first[lo] <= i, and hi == B or first[hi] > i
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+HX_DEVINL int pages_of(long long tokens, int S) { return (int)((tokens + S - 1) / S); }
+
+struct ExtendParams {
+  int32_t* table;
+  int64_t stride;
+  int B, W, S;
+  const int32_t* cached;
+  const int32_t* fresh;
+  const int32_t* free_pages;
+  int64_t free_cap;
+  const int32_t* free_count;
+  int32_t* refs;
+  int num_pages;
+  int32_t* query_start;
+  int32_t* seq_lens;
+  int64_t* slots;
+  int64_t* positions;
+  int num_tokens;
+  int32_t* free_out;
+  uint32_t* err;
+};
+
+__global__ void __launch_bounds__(NT) extend_kernel(const ExtendParams p) {
+  extern __shared__ int smem[];
+  int* qs = smem;            // first token of each sequence
+  int* pf = smem + p.B;      // first new page of each sequence
+  __shared__ long long ws[NT / 32][2];
+  __shared__ uint32_t bad;
+  const int tid = threadIdx.x;
+  if (tid == 0) bad = 0u;
+  __syncthreads();
+  // ---- prefix sums of new tokens and new pages, and the checks: the same in every CTA
+  const int per = (p.B + NT - 1) / NT, b0 = tid * per, b1 = min(p.B, b0 + per);
+  long long st = 0, sp = 0;
+  uint32_t mine = 0u;
+  for (int b = b0; b < b1; ++b) {
+    const long long c = p.cached[b], n = p.fresh[b];
+    if (c < 0 || n < 0 || (c + n + p.S - 1) / p.S > p.W) {
+      mine = HX_DEV_ERR_BOUNDS;
+      continue;
+    }
+    st += n;
+    sp += pages_of(c + n, p.S) - pages_of(c, p.S);
+  }
+  long long it = st, ip = sp, tt, tp;
+  block_scan2<NT>(it, ip, tt, tp, ws);
+  const long long count = *p.free_count;
+  if (mine) atomicOr(&bad, mine);
+  if (tid == 0) {
+    if (tt > p.num_tokens || count < 0 || count > p.free_cap) atomicOr(&bad, HX_DEV_ERR_BOUNDS);
+    else if (tp > count) atomicOr(&bad, HX_DEV_ERR_PAGES);
+  }
+  __syncthreads();
+  const uint32_t fail = bad;
+  if (!fail) {
+    int t = (int)(it - st), q = (int)(ip - sp);
+    for (int b = b0; b < b1; ++b) {
+      const int c = p.cached[b], n = p.fresh[b];
+      qs[b] = t;
+      pf[b] = q;
+      t += n;
+      q += pages_of((long long)c + n, p.S) - pages_of(c, p.S);
+    }
+  }
+  __syncthreads();
+  const int total = fail ? 0 : (int)tt, fresh_pages = fail ? 0 : (int)tp;
+  if (blockIdx.x == 0) {
+    for (int b = tid; b < p.B; b += NT) {
+      p.query_start[b] = fail ? 0 : qs[b];
+      p.seq_lens[b] = p.cached[b] + (fail ? 0 : p.fresh[b]);
+    }
+    if (tid == 0) {
+      p.query_start[p.B] = total;
+      *p.free_out = (int32_t)(count - fresh_pages);
+      if (fail) set_err(p.err, fail);
+    }
+  }
+  // ---- new pages: table entries and reference counts
+  for (int k = blockIdx.x * NT + tid; k < fresh_pages; k += gridDim.x * NT) {
+    const int b = find_row(pf, p.B, k);
+    const int j = pages_of(p.cached[b], p.S) + k - pf[b];
+    const int page = p.free_pages[count - 1 - k];
+    if (page < 0 || page >= p.num_pages) {
+      set_err(p.err, HX_DEV_ERR_BOUNDS);
+      continue;
+    }
+    p.table[(int64_t)b * p.stride + j] = page;
+    if (p.refs) p.refs[page] = 1;
+  }
+  // ---- tokens: slot and position; rows past the batch get slot -1 (skipped by the pack) and position 0
+  for (int i = blockIdx.x * NT + tid; i < p.num_tokens; i += gridDim.x * NT) {
+    int64_t slot = -1, pos = 0;
+    if (i < total) {
+      const int b = find_row(qs, p.B, i);
+      const int c = p.cached[b];
+      pos = (int64_t)c + i - qs[b];
+      const int j = (int)(pos / p.S), have = pages_of(c, p.S);
+      const int page = j < have ? p.table[(int64_t)b * p.stride + j] : p.free_pages[count - 1 - (pf[b] + j - have)];
+      if (page < 0 || page >= p.num_pages) set_err(p.err, HX_DEV_ERR_BOUNDS);
+      else slot = (int64_t)page * p.S + pos % p.S;
+    }
+    p.slots[i] = slot;
+    p.positions[i] = pos;
+  }
+}
+
+struct TruncateParams {
+  const int32_t* table;
+  int64_t stride;
+  int B, W, S;
+  const int32_t* lens;
+  const int32_t* keep;
+  int32_t* free_pages;
+  int64_t free_cap;
+  const int32_t* free_count;
+  int32_t* refs;
+  int num_pages;
+  int32_t* lens_out;
+  int32_t* free_out;
+  uint32_t* err;
+};
+
+// Drops pages [ceil(keep / S), ceil(len / S)) of every sequence. Dropped
+// entries are numbered k sequence by sequence and pushed in reverse, so that
+// truncating what extend just added leaves the stack as it was. With
+// reference counts an entry takes one reference; a page whose last reference
+// goes is pushed once, at the place of the call's last entry naming it (the
+// order does not depend on which thread's atomic came first):
+//   1  each entry takes a reference by compare-and-swap; the one that takes the
+//      last leaves INT_MIN in place of 0. An entry that finds no reference is
+//      an error and takes nothing
+//   2  entries of pages at INT_MIN raise it to INT_MIN + 1 + k (atomicMax)
+//   3  the entry that finds its own mark pushes the page; the mark becomes 0
+__global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
+  extern __shared__ int smem[];
+  int* pf = smem;
+  __shared__ long long ws[NTT / 32][2];
+  __shared__ uint32_t bad;
+  __shared__ int freed, run;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) bad = 0u, freed = 0, run = 0;
+  __syncthreads();
+  const int per = (p.B + NTT - 1) / NTT, b0 = tid * per, b1 = min(p.B, b0 + per);
+  long long sp = 0, dummy = 0, tp, td;
+  uint32_t mine = 0u;
+  for (int b = b0; b < b1; ++b) {
+    const long long n = p.lens[b], k = max(0, min(p.keep[b], p.lens[b]));
+    if (n < 0 || (n + p.S - 1) / p.S > p.W) mine = HX_DEV_ERR_BOUNDS;
+    else sp += pages_of(n, p.S) - pages_of(k, p.S);
+  }
+  long long ip = sp;
+  block_scan2<NTT>(ip, dummy, tp, td, ws);
+  const long long count = *p.free_count;
+  if (mine) atomicOr(&bad, mine);
+  if (tid == 0 && (count < 0 || count > p.free_cap || tp > 0x7ffffff0ll || (!p.refs && count + tp > p.free_cap)))
+    atomicOr(&bad, HX_DEV_ERR_BOUNDS);
+  __syncthreads();
+  if (bad) {  // nothing is given back
+    for (int b = tid; b < p.B; b += NTT) p.lens_out[b] = p.lens[b];
+    if (tid == 0) {
+      *p.free_out = (int32_t)count;
+      set_err(p.err, bad);
+    }
+    return;
+  }
+  int q = (int)(ip - sp);
+  for (int b = b0; b < b1; ++b) {
+    pf[b] = q;
+    q += pages_of(p.lens[b], p.S) - pages_of(max(0, min(p.keep[b], p.lens[b])), p.S);
+  }
+  __syncthreads();
+  const int total = (int)tp;
+  auto entry = [&](int k) -> int {
+    const int b = find_row(pf, p.B, k);
+    const int j = pages_of(max(0, min(p.keep[b], p.lens[b])), p.S) + k - pf[b];
+    const int page = p.table[(int64_t)b * p.stride + j];
+    if (page >= 0 && page < p.num_pages) return page;
+    set_err(p.err, HX_DEV_ERR_BOUNDS);
+    return -1;
+  };
+  constexpr int kMark = (int)0x80000000;
+  if (!p.refs) {
+    for (int k = tid; k < total; k += NTT) p.free_pages[count + total - 1 - k] = entry(k);
+  } else {
+    int here = 0;
+    for (int k = tid; k < total; k += NTT) {
+      const int page = entry(k);
+      if (page < 0) continue;
+      int old = p.refs[page];
+      while (old > 0) {
+        const int seen = atomicCAS(p.refs + page, old, old == 1 ? kMark : old - 1);
+        if (seen == old) break;
+        old = seen;
+      }
+      if (old <= 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
+      here += old == 1;
+    }
+    if (here) atomicAdd(&freed, here);
+    __syncthreads();
+    const int n_free = freed;
+    const bool fits = count + n_free <= p.free_cap;
+    if (!fits && tid == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
+    for (int k = tid; k < total; k += NTT) {
+      const int page = entry(k);
+      if (page >= 0 && __ldcg(p.refs + page) < 0) atomicMax(p.refs + page, kMark + 1 + k);
+    }
+    __syncthreads();
+    for (int k0 = 0; k0 < total; k0 += NTT) {  // ranks by a running block scan, chunk by chunk
+      const int k = k0 + tid;
+      const int page = k < total ? entry(k) : -1;
+      const bool mine_now = page >= 0 && __ldcg(p.refs + page) == kMark + 1 + k;
+      const uint32_t m = __ballot_sync(0xffffffffu, mine_now);
+      if (lane == 0) ws[warp][0] = __popc(m);
+      __syncthreads();
+      int before = run, all = 0;
+      for (int w = 0; w < NTT / 32; ++w) {
+        if (w < warp) before += (int)ws[w][0];
+        all += (int)ws[w][0];
+      }
+      if (mine_now) {
+        const int rank = before + __popc(m & ((1u << lane) - 1u));
+        if (fits) p.free_pages[count + n_free - 1 - rank] = page;
+        p.refs[page] = 0;
+      }
+      __syncthreads();
+      if (tid == 0) run += all;
+      __syncthreads();
+    }
+    if (!fits && tid == 0) freed = 0;
+    __syncthreads();
+  }
+  for (int b = tid; b < p.B; b += NTT) p.lens_out[b] = max(0, min(p.keep[b], p.lens[b]));
+  if (tid == 0) *p.free_out = (int32_t)(count + (p.refs ? freed : total));
+}
+
+// Empties pages[lo .. hi) (lo, hi read on the device) as hx_pool_reset_pages does.
+__global__ void reset_range_kernel(hx_pool_layer pool, const int32_t* pages, int64_t cap, const int32_t* lo_p,
+                                   const int32_t* hi_p, uint32_t* err) {
+  const int h = blockIdx.y, D = pool.head_size;
+  const int64_t lo = *lo_p, hi = *hi_p;
+  if (lo < 0 || hi > cap) {
+    if (threadIdx.x == 0) set_err(err, HX_DEV_ERR_BOUNDS);
+    return;
+  }
+  for (int64_t i = lo + blockIdx.x; i < hi; i += gridDim.x) {
+    const int pg = pages[i];
+    if (pg < 0 || pg >= pool.num_blocks) {
+      if (threadIdx.x == 0) set_err(err, HX_DEV_ERR_BOUNDS);
+      continue;
+    }
+    uint16_t* st = pool.stats + ((int64_t)h * pool.num_blocks + pg) * 2 * D;
+    for (int d = threadIdx.x; d < 2 * D; d += blockDim.x) st[d] = d < D ? 0x7C00u : 0xFC00u;
+    if (threadIdx.x < 2) {
+      uint32_t* dr = pool.dir + (((int64_t)h * pool.num_blocks + pg) * 2 + threadIdx.x) * 4;
+      dr[2] = 0;
+      dr[3] = 0;
+    }
+  }
+}
+
+}  // namespace pg
+}  // namespace hx
+
+using namespace hx;
+
+extern "C" {
+
+HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_stride, int32_t B, int32_t max_pages,
+                            int32_t page_size, const int32_t* cached_lens, const int32_t* new_tokens,
+                            const int32_t* free_pages, int64_t free_capacity, const int32_t* free_count,
+                            int32_t* page_refs, int32_t num_pages, int32_t* query_start, int32_t* seq_lens,
+                            int64_t* slot_mapping, int64_t* positions, int32_t num_tokens, int32_t* free_count_out,
+                            uint32_t* dev_err) {
+  if (B < 0 || max_pages < 0 || page_size < 1 || num_pages < 0 || num_tokens < 0 || free_capacity < 0)
+    return HX_ERR_ARG;
+  if (!query_start || !free_count || !free_count_out || free_count == free_count_out) return HX_ERR_ARG;
+  if (B > 0 && (!block_table || !cached_lens || !new_tokens || !seq_lens || bt_stride < max_pages)) return HX_ERR_ARG;
+  if (B > 0 && (seq_lens == cached_lens || seq_lens == new_tokens)) return HX_ERR_ARG;
+  if ((num_tokens > 0 && (!slot_mapping || !positions)) || (free_capacity > 0 && !free_pages)) return HX_ERR_ARG;
+  if (B > pg::MAXB) return HX_ERR_UNSUPPORTED;
+  pg::ExtendParams p{block_table, bt_stride,   B,        max_pages,   page_size, cached_lens,  new_tokens,
+                     free_pages,  free_capacity, free_count, page_refs, num_pages, query_start, seq_lens,
+                     slot_mapping, positions,   num_tokens, free_count_out, dev_err};
+  const size_t smem = (size_t)2 * (B > 0 ? B : 1) * sizeof(int);
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(pg::extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return HX_ERR_LAUNCH;
+  }
+  int grid = (num_tokens + pg::kTokensPerCta - 1) / pg::kTokensPerCta;
+  grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
+  pg::extend_kernel<<<grid, pg::NT, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  HX_LAUNCH_CHECK();
+  return HX_OK;
+}
+
+HX_API int hx_tables_truncate(void* stream, const int32_t* block_table, int64_t bt_stride, int32_t B,
+                              int32_t max_pages, int32_t page_size, const int32_t* seq_lens,
+                              const int32_t* keep_lens, int32_t* free_pages, int64_t free_capacity,
+                              const int32_t* free_count, int32_t* page_refs, int32_t num_pages, int32_t* seq_lens_out,
+                              int32_t* free_count_out, uint32_t* dev_err) {
+  if (B < 0 || max_pages < 0 || page_size < 1 || num_pages < 0 || free_capacity < 0) return HX_ERR_ARG;
+  if (!free_count || !free_count_out || (free_capacity > 0 && !free_pages)) return HX_ERR_ARG;
+  if (B > 0 && (!block_table || !seq_lens || !keep_lens || !seq_lens_out || bt_stride < max_pages)) return HX_ERR_ARG;
+  if (B > pg::MAXB) return HX_ERR_UNSUPPORTED;
+  pg::TruncateParams p{block_table, bt_stride,  B,         max_pages, page_size,    seq_lens,       keep_lens, free_pages,
+                       free_capacity, free_count, page_refs, num_pages, seq_lens_out, free_count_out, dev_err};
+  const size_t smem = (size_t)(B > 0 ? B : 1) * sizeof(int);
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(pg::truncate_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)smem) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return HX_ERR_LAUNCH;
+  }
+  pg::truncate_kernel<<<1, pg::NTT, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  HX_LAUNCH_CHECK();
+  return HX_OK;
+}
+
+HX_API int hx_pool_reset_range(void* stream, const hx_pool_layer* pool, const int32_t* pages, int64_t capacity,
+                               const int32_t* begin, const int32_t* end, uint32_t* dev_err) {
+  if (!pool || !pages || !begin || !end || capacity < 0) return HX_ERR_ARG;
+  if (!pool->stats || !pool->dir || pool->num_kv_heads < 1 || pool->num_kv_heads > 65535 || pool->head_size < 1)
+    return HX_ERR_ARG;
+  if (capacity == 0) return HX_OK;
+  const int64_t gx = capacity < 592 ? capacity : 592;  // 4 blocks an SM, striding over the range
+  pg::reset_range_kernel<<<dim3((unsigned)gx, pool->num_kv_heads), 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      *pool, pages, capacity, begin, end, dev_err);
+  HX_LAUNCH_CHECK();
+  return HX_OK;
+}
+
+}  // extern "C"

@@ -19,7 +19,7 @@ LIB_PATH = Path(os.environ.get("HELIX_KV_LIB", _HERE / "libhelix_kv.so"))
 # status and device error bits (helix_kv.h)
 HX_OK, HX_ERR_ARG, HX_ERR_UNSUPPORTED, HX_ERR_LAUNCH, HX_ERR_SCRATCH_LIMIT = 0, 1, 2, 3, 4
 DEV_ERR = {0x1: "outlier arena full", 0x2: "index out of range", 0x4: "bounded wait ran out",
-           0x8: "selection threshold not isolated"}
+           0x8: "selection threshold not isolated", 0x10: "too few free pages"}
 SEL_DENSE, SEL_THRESHOLD, SEL_LIST, SEL_SLICES = 0, 1, 2, 3
 VPOS_PHYSICAL = 0x100  # OR-ed into the decode's sel_mode (helix_kv.h)
 DECODE_CUDA_CORES = 0x200  # OR-ed into sel_mode: QK and PV in FFMA (helix_kv.h)
@@ -45,6 +45,11 @@ _SIGS = {
     "hx_version": (ctypes.c_char_p, []),
     "hx_pool_init": (c_i32, [c_vp, _P(PoolLayer)]),
     "hx_pool_reset_pages": (c_i32, [c_vp, _P(PoolLayer), c_vp, c_i32, c_vp]),
+    "hx_pool_reset_range": (c_i32, [c_vp, _P(PoolLayer), c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "hx_tables_extend": (c_i32, [c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32,
+                                 c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "hx_tables_truncate": (c_i32, [c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32,
+                                   c_vp, c_vp, c_vp]),
     "hx_pack_append": (c_i32, [c_vp, _P(PoolLayer), _P(LayerScales), c_vp, c_vp, c_vp, c_vp, c_i32, c_vp]),
     "hx_scales_prepare": (c_i32, [c_vp, _P(LayerScales), c_i32, c_i32, c_vp, c_vp]),
     "hx_unpack_pages": (c_i32, [c_vp, _P(PoolLayer), _P(LayerScales), c_vp, c_vp, c_i32, c_vp, c_vp, c_vp]),
@@ -123,7 +128,7 @@ LAUNCHES = {"hx_scales_prepare": 2, "hx_pool_init": 1, "hx_pool_reset_pages": 1,
             "hx_nuq_dequantize_flat": 1, "hx_page_stats": 1, "hx_quest_scores": 1, "hx_quest_threshold": lambda a: 1 if a[11] else 2,
             "hx_quest_threshold_slices": lambda a: 1 if a[11] else 2, "hx_quest_localize": 1,
             "hx_quest_compact": 1, "hx_quest_lists": 2, "hx_decode_attn": 1, "hx_decode_attn_noalloc": 1, "hx_prefill_attn": 1, "hx_calib_rows": 1, "hx_decode_attn_select": 1, "hx_merge_partials": 1, "hx_merge_gathered": 1, "hx_exchange_merge": 1,
-            "hx_selected_attention": 1}
+            "hx_selected_attention": 1, "hx_pool_reset_range": 1, "hx_tables_extend": 1, "hx_tables_truncate": 1}
 launch_count = [0]
 
 

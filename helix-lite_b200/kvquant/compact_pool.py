@@ -128,6 +128,19 @@ class CompactKVPool:
             call("hx_pool_reset_pages", stream(self.device), ctypes_ref(self.layers[layer_idx].struct), ptr(p),
                  p.numel(), ptr(hxlib.err_word(self.device)))
 
+    def reset_allocated(self, layer_idx: int, free_pages: torch.Tensor, count_before: torch.Tensor,
+                        count_after: torch.Tensor) -> None:
+        """Empty the pages that one ``paging.extend_tables`` call took off the
+        stack ``free_pages``: entries [count_after, count_before), both (1,)
+        int32 device counts (its ``free_count`` argument and result)."""
+        hxlib.require_cuda(free_pages, count_before, count_after)
+        for t in (free_pages, count_before, count_after):
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.layers[layer_idx].stats.device:
+                raise ValueError("reset_allocated takes contiguous int32 tensors on the pool's device")
+        with torch.cuda.device(self.device):
+            call("hx_pool_reset_range", stream(self.device), ctypes_ref(self.layers[layer_idx].struct), ptr(free_pages),
+                 free_pages.numel(), ptr(count_after), ptr(count_before), ptr(hxlib.err_word(self.device)))
+
     def check(self) -> None:
         """Synchronise and raise if a kernel flagged a device error."""
         hxlib.check_device_errors(self.device)

@@ -49,6 +49,7 @@ extern "C" {
 #define HX_DEV_ERR_BOUNDS     0x2u  /* an index (page, slot, level) out of range */
 #define HX_DEV_ERR_TIMEOUT    0x4u  /* a bounded wait on a bulk copy ran out */
 #define HX_DEV_ERR_SELECT     0x8u  /* selection could not isolate a threshold */
+#define HX_DEV_ERR_PAGES      0x10u /* too few free pages for a batch's tables  */
 
 /* Calibrated nuq scales of one layer (src/kvquant/scales.py:14-70). */
 typedef struct hx_layer_scales {
@@ -102,6 +103,55 @@ HX_API int hx_pool_init(void* stream, const hx_pool_layer* pool);
 /* Empty the listed pages (stats and outlier lists) so they can be reused. */
 HX_API int hx_pool_reset_pages(void* stream, const hx_pool_layer* pool,
                                const int32_t* pages, int32_t n, uint32_t* dev_err);
+
+/* Empty pages[*begin .. *end) (device counters, 0 <= *begin, *end <= capacity):
+ * the pages one hx_tables_extend handed out are free_pages[free_count_out ..
+ * free_count). One kernel; no reference counterpart. */
+HX_API int hx_pool_reset_range(void* stream, const hx_pool_layer* pool, const int32_t* pages, int64_t capacity,
+                               const int32_t* begin, const int32_t* end, uint32_t* dev_err);
+
+/* ---- block tables and slot maps --------------------------------------- */
+
+/*
+ * Room for new_tokens[b] more tokens in each of B sequences (at most 16384).
+ * A sequence of c = cached_lens[b] tokens holds table entries [0, ceil(c / S))
+ * of row block_table + b * bt_stride (max_pages entries) and gets those up to
+ * ceil((c + new) / S): the k-th new page of the call, sequence by sequence, is
+ * free_pages[*free_count - 1 - k]. Writes those entries, page_refs[page] = 1
+ * for each (when non-NULL), query_start (B + 1, exclusive prefix of
+ * new_tokens), seq_lens = c + new, and for the num_tokens rows of the slot map
+ * slot_mapping = page * S + position % S and positions; rows past the batch's
+ * tokens get slot -1 (hx_pack_append skips them) and position 0;
+ * *free_count_out = pages left. Page ids must lie in [0, num_pages)
+ * (HX_DEV_ERR_BOUNDS, slot -1). A negative length, a sequence past max_pages or
+ * more than num_tokens tokens (HX_DEV_ERR_BOUNDS), or too few free pages
+ * (HX_DEV_ERR_PAGES) hand out nothing: slots -1, query_start 0, seq_lens =
+ * cached_lens, count unchanged. Outputs must not overlap inputs. One kernel.
+ * No reference counterpart (vLLM's scheduler builds these on the host).
+ */
+HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_stride, int32_t B, int32_t max_pages,
+                            int32_t page_size, const int32_t* cached_lens, const int32_t* new_tokens,
+                            const int32_t* free_pages, int64_t free_capacity, const int32_t* free_count,
+                            int32_t* page_refs, int32_t num_pages, int32_t* query_start, int32_t* seq_lens,
+                            int64_t* slot_mapping, int64_t* positions, int32_t num_tokens, int32_t* free_count_out,
+                            uint32_t* dev_err);
+
+/*
+ * The way back: sequence b keeps min(keep_lens[b], seq_lens[b]) tokens
+ * (seq_lens_out) and its entries [ceil(keep / S), ceil(len / S)) are dropped.
+ * Dropped entry k of N, sequence by sequence, goes to free_pages[*free_count +
+ * N - 1 - k], so truncating what hx_tables_extend just added restores the
+ * stack. With page_refs an entry gives back one reference; a page is pushed
+ * once, when its last reference goes, in the order of the call's last entries
+ * naming each freed page. *free_count_out = pages on the stack. A page without
+ * a reference, an id outside [0, num_pages), bad lengths or a full stack are
+ * HX_DEV_ERR_BOUNDS. One kernel. No reference counterpart.
+ */
+HX_API int hx_tables_truncate(void* stream, const int32_t* block_table, int64_t bt_stride, int32_t B,
+                              int32_t max_pages, int32_t page_size, const int32_t* seq_lens,
+                              const int32_t* keep_lens, int32_t* free_pages, int64_t free_capacity,
+                              const int32_t* free_count, int32_t* page_refs, int32_t num_pages,
+                              int32_t* seq_lens_out, int32_t* free_count_out, uint32_t* dev_err);
 
 /* ---- pack on write (Kernel A) ----------------------------------------- */
 
