@@ -1,0 +1,482 @@
+// Causal attention over whole prompts, packed back to back, grouped heads.
+//
+//   s_ij = scale * q_i . k_j  (j <= i, same sequence),  o_i = sum_j softmax(s_i)_j v_j,
+//   lse_i = log sum_j exp(s_ij)
+//
+// One CTA = (two tiles of 128 query rows, KV head, sequence). A row is one
+// (token, head of the group) pair, TQ = 128 / G tokens a tile, so all heads of
+// a group share the K and V tiles and short prompts fill the tiles' rows. Keys
+// stream in tiles of 128. Per tile and key tile:
+//   S = Q K^T    tcgen05.mma, both operands in shared memory (tensor-map loads,
+//                128-byte swizzle), S (128 x 128 fp32) in TMEM
+//   P            a warpgroup holds one row of S a thread: running maximum and
+//                sum in fp32 (exp2 domain), P rounded to the inputs' type (the
+//                matrix unit's operand; the sum keeps the fp32 values) and
+//                stored over S in TMEM. The maximum used for P moves only when
+//                a score passes it by 2^8, so O is rescaled rarely
+//   O += P V     tcgen05.mma, P from TMEM, V from shared memory
+// The two query tiles alternate on the tensor core: one tile's products run
+// under the other's softmax. The products of a tile are issued in the order
+// PV(i), S(i + 1), so that S(i + 1) complete means O(i) complete.
+//
+// Masked places: a masked score is replaced by -inf, never added to, so K there
+// may hold anything. V there meets P = 0 in the product, and 0 * inf is NaN: in
+// the key tiles that hold masked places two warps replace rows past the
+// sequence's end and non-finite values by 0 before the product, and rows
+// allowed to see a non-finite value get it added at the end (P > 0 there).
+#include "tcgen.cuh"
+
+namespace hx {
+namespace pr {
+
+constexpr int NTHREADS = 384;   // 2 softmax warpgroups; MMA, load and 2 V-check warps
+constexpr int STAGES = 5;       // K and V tiles in flight
+constexpr int KT = 128;         // keys per tile
+constexpr int ROWS = 128;       // query rows per tile
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.0f;  // P <= 2^8 before the maximum moves
+
+template <int D>
+struct Smem {
+  alignas(1024) uint8_t q[2][ROWS * D * 2];
+  alignas(1024) uint8_t kv[STAGES][KT * D * 2];
+  uint64_t q_full[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], v_go, v_clean, drain;
+  uint32_t tmem, abort, bad_v;
+};
+
+struct Params {
+  CUtensorMap mq, mk, mv;
+  const int32_t* start;
+  int B, T, H, G, TQ;
+  float c;  // softmax scale * log2 e
+  const uint16_t* v;
+  int64_t v_st, v_sh;
+  uint16_t* out;
+  float* lse;
+  uint32_t* err;
+};
+
+// Work item of a slot. Sequence b's tiles are slots f(b) .. f(b) + ceil(len / n)
+// - 1 with f(b) = floor(start_b / n) + b, n tokens a CTA: ceil(len_b / n) <=
+// floor(start_{b+1} / n) - floor(start_b / n) + 1, so slots never meet and no
+// prefix sum over the batch is needed; floor(T / n) + B slots hold all. b is the
+// last with f(b) <= slot, found by the warp 32 candidates at a time.
+HX_DEVINL int find_seq(const int32_t* start, int B, int n, int slot) {
+  const int lane = lane_id();
+  int lo = 0, hi = B;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int b = lo + lane * step;
+    const bool le = b < hi && start[b] / n + b <= slot;
+    const uint32_t m = __ballot_sync(0xffffffffu, le);
+    const int last = m ? 31 - __clz(m) : 0;
+    lo += last * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+template <bool BF16>
+HX_DEVINL uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// bits of the 16-bit halves whose value is not finite
+template <bool BF16>
+HX_DEVINL uint32_t nonfinite2(uint32_t x) {
+  constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
+  return ((x & e) == e ? 0xFFFFu : 0u) | (((x >> 16) & e) == e ? 0xFFFF0000u : 0u);
+}
+template <bool BF16>
+HX_DEVINL float to_float(uint16_t x) {
+  return BF16 ? __uint_as_float((uint32_t)x << 16) : h2f(x);
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t raw[];
+  Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x % p.H, slot = (int)(gridDim.x / p.H) - 1 - (int)(blockIdx.x / p.H);
+  const int TQ = p.TQ, G = p.G, per = 2 * TQ;
+  const int b = find_seq(p.start, p.B, per, slot);
+  const int s0 = p.start[b], len = p.start[b + 1] - s0;
+  if (s0 < 0 || len < 0 || s0 + len > p.T) {
+    if (threadIdx.x == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
+    return;
+  }
+  const int t0 = (slot - s0 / per - b) * per;  // first token of the CTA, in the sequence
+  if (t0 < 0 || t0 >= len) return;
+  const int nq = t0 + TQ < len ? 2 : 1;        // query tiles with tokens
+  const int n = (min(t0 + per, len) + KT - 1) / KT;
+  const int i_mask = min((t0 + 1) / KT, n - 1);  // first key tile with masked places
+
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int q = 0; q < 2; ++q) {
+        mbar_init(&sm.q_full[q], 1);
+        mbar_init(&sm.s_full[q], 1);
+        mbar_init(&sm.p_full[q], 4);
+        mbar_init(&sm.o_full[q], 1);
+      }
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&sm.kv_full[s], 1);
+        mbar_init(&sm.kv_empty[s], 1);
+      }
+      mbar_init(&sm.v_go, 1);
+      mbar_init(&sm.v_clean, 2);
+      mbar_init(&sm.drain, 1);
+      sm.abort = 0u;
+      sm.bad_v = 0u;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tc::tmem_alloc(&sm.tmem, 512);
+  }
+  if (warp == 9 && lane == 0) {
+    tc::prefetch_map(&p.mq);
+    tc::prefetch_map(&p.mk);
+    tc::prefetch_map(&p.mv);
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sm.tmem;
+  volatile uint32_t* abort = &sm.abort;
+  constexpr int HALF = KT * 128;  // bytes of 128 rows of 64 elements
+  constexpr int NH = D / 64;
+
+  if (warp < 8) {
+    // ---- softmax: warpgroup q holds tile q's rows, one a thread
+    tc::regs_inc<216>();
+    const int q = warp >> 2, r = threadIdx.x & 127;
+    if (q < nq) {
+      const int ti = t0 + q * TQ + r / G;          // token of the row, in the sequence
+      const bool live = r < TQ * G && ti < len;
+      const int tile0 = t0 + q * TQ;               // lowest position of the tile
+      const uint32_t sb = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * q;
+      const uint32_t ob = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 + 128 * q;
+      float m = -INFINITY, l = 0.0f;
+      bool ok = true;
+      for (int i = 0; i < n && ok; ++i) {
+        ok = tc::wait_warp(&sm.s_full[q], i & 1, abort);
+        if (!ok) break;
+        tc::fence_after();
+        uint32_t s[KT];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) tc::ld32(s + 32 * u, sb + 32 * u);
+        tc::wait_ld();
+        if (KT * i + KT - 1 > tile0) {  // masked places: keys past the row's position
+          const int lim = ti - KT * i;
+#pragma unroll
+          for (int j = 0; j < KT; ++j) s[j] = j <= lim ? s[j] : 0xff800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < KT; j += 8)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            mx[u] = fmaxf(mx[u], fmaxf(__uint_as_float(s[j + 2 * u]), __uint_as_float(s[j + 2 * u + 1])));
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const bool move = (mt - m) * p.c > kSlack;  // also the first finite maximum (m = -inf)
+        if (__any_sync(0xffffffffu, move)) {
+          const float mn = move ? mt : m;
+          const float a = move ? tc::ex2((m - mn) * p.c) : 1.0f;
+          m = mn;
+          l *= a;
+          if (i > 0) {  // O(i - 1) is complete: S(i) was issued after it
+            const uint64_t a2 = tc::f2_pack(a, a);
+#pragma unroll 1
+            for (int u = 0; u < D / 32; ++u) {
+              uint32_t o[32];
+              tc::ld32(o, ob + 32 * u);
+              tc::wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                float x, y;
+                tc::f2_unpack(tc::f2_mul(tc::f2_pack(__uint_as_float(o[j]), __uint_as_float(o[j + 1])), a2), x, y);
+                o[j] = __float_as_uint(x);
+                o[j + 1] = __float_as_uint(y);
+              }
+              tc::st32(ob + 32 * u, o);
+            }
+          }
+        }
+        const float mb = m == -INFINITY ? 0.0f : -m * p.c;
+        const uint64_t c2 = tc::f2_pack(p.c, p.c), mb2 = tc::f2_pack(mb, mb);
+        uint64_t sum[2] = {0ull, 0ull};
+        uint32_t pk[KT / 2];
+#pragma unroll
+        for (int j = 0; j < KT; j += 2) {
+          float x, y;
+          tc::f2_unpack(tc::f2_fma(tc::f2_pack(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), c2, mb2), x, y);
+          x = tc::ex2(x);
+          y = tc::ex2(y);
+          sum[(j >> 1) & 1] = tc::f2_add(sum[(j >> 1) & 1], tc::f2_pack(x, y));
+          pk[j >> 1] = pack2<BF16>(x, y);
+        }
+        tc::st32(sb, pk);
+        tc::st32(sb + 32, pk + 32);
+        {
+          float x, y;
+          tc::f2_unpack(tc::f2_add(sum[0], sum[1]), x, y);
+          l += x + y;
+        }
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::arrive(&sm.p_full[q]);
+      }
+      // ---- O / l
+      if (ok) ok = tc::wait_warp(&sm.o_full[q], 0, abort);
+      tc::fence_after();
+      if (ok) {
+        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+        const int64_t row = ((int64_t)(s0 + ti) * p.H + h) * G + r % G;
+        const bool bad = sm.bad_v != 0u;
+#pragma unroll 1
+        for (int u = 0; u < D / 32; ++u) {
+          uint32_t o[32];
+          tc::ld32(o, ob + 32 * u);
+          tc::wait_ld();
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(o[j]) * inv;
+          if (bad && live) {  // non-finite V that the row sees in the masked tiles
+            for (int key = i_mask * KT; key <= ti; ++key) {
+              const uint16_t* vr = p.v + (int64_t)(s0 + key) * p.v_st + h * p.v_sh + 32 * u;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float x = to_float<BF16>(vr[j]);
+                if (!(fabsf(x) < INFINITY)) f[j] += x;
+              }
+            }
+          }
+          if (live) {
+            uint4* dst = reinterpret_cast<uint4*>(p.out + row * D + 32 * u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              dst[j] = make_uint4(pack2<BF16>(f[8 * j], f[8 * j + 1]), pack2<BF16>(f[8 * j + 2], f[8 * j + 3]),
+                                  pack2<BF16>(f[8 * j + 4], f[8 * j + 5]), pack2<BF16>(f[8 * j + 6], f[8 * j + 7]));
+          }
+        }
+        if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m * p.c + log2f(l)) * kLn2;
+      }
+    }
+  } else {
+    tc::regs_dec<72>();
+    if (warp == 8) {
+      // ---- matrix products (one thread issues)
+      constexpr uint32_t ids = tc::idesc_f16(BF16, ROWS, KT, 0), idv = tc::idesc_f16(BF16, ROWS, D, 1);
+      auto qk = [&](int q, int stage) {
+        const uint32_t qa = smem_u32(sm.q[q]), ka = smem_u32(sm.kv[stage]);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k / 4) * HALF + (k % 4) * 32;
+          tc::mma_ss(tmem + 128 * q, tc::desc128(qa + off, 0), tc::desc128(ka + off, 0), ids, k > 0);
+        }
+        tc::commit(&sm.s_full[q]);
+      };
+      bool ok = tc::wait_warp(&sm.kv_full[0], 0, abort);
+      for (int q = 0; q < nq && ok; ++q) {
+        ok = tc::wait_warp(&sm.q_full[q], 0, abort);
+        if (ok && lane == 0) qk(q, 0);
+        __syncwarp();
+      }
+      if (ok && lane == 0) tc::commit(&sm.kv_empty[0]);
+      for (int i = 0; i < n && ok; ++i) {
+        const int cv = 2 * i + 1, ck = 2 * i + 2, sv = cv % STAGES, sk = ck % STAGES;
+        ok = tc::wait_warp(&sm.kv_full[sv], (cv / STAGES) & 1, abort);
+        if (ok && i >= i_mask && lane == 0) tc::arrive(&sm.v_go);
+        if (ok && i + 1 < n) ok = tc::wait_warp(&sm.kv_full[sk], (ck / STAGES) & 1, abort);
+        const uint32_t va = smem_u32(sm.kv[sv]);
+        for (int q = 0; q < nq && ok; ++q) {
+          ok = tc::wait_warp(&sm.p_full[q], i & 1, abort);
+          if (ok && q == 0 && i >= i_mask) ok = tc::wait_warp(&sm.v_clean, (i - i_mask) & 1, abort);
+          if (ok && lane == 0) {
+            tc::fence_after();
+#pragma unroll
+            for (int k = 0; k < KT / 16; ++k)
+              tc::mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * k, tc::desc128(va + 2048 * k, HALF), idv,
+                         i > 0 || k > 0);
+            if (i + 1 < n) qk(q, sk);
+            else tc::commit(&sm.o_full[q]);
+          }
+          __syncwarp();
+        }
+        if (ok && lane == 0) {
+          tc::commit(&sm.kv_empty[sv]);
+          if (i + 1 < n) tc::commit(&sm.kv_empty[sk]);
+        }
+        __syncwarp();
+      }
+      if (lane == 0) tc::commit(&sm.drain);  // no product may be in flight when TMEM is freed
+      __syncwarp();
+      (void)mbar_wait(&sm.drain, 0);
+    } else if (warp == 9) {
+      // ---- loads: Q tiles, then K0 V0 K1 V1 ...
+      bool ok = true;
+      int c = 0;
+      if (lane == 0) {
+        auto load = [&](const CUtensorMap* map, int key) {
+          const int s = c % STAGES;
+          if (c >= STAGES) ok = tc::wait(&sm.kv_empty[s], ((c / STAGES) & 1) ^ 1, abort);
+          if (!ok) return;
+          mbar_arrive_expect_tx(&sm.kv_full[s], KT * D * 2);
+#pragma unroll
+          for (int u = 0; u < NH; ++u) tc::tma3(sm.kv[s] + u * HALF, map, 64 * u, h, s0 + key, &sm.kv_full[s]);
+          ++c;
+        };
+        auto load_q = [&](int q) {
+          mbar_arrive_expect_tx(&sm.q_full[q], TQ * G * D * 2);
+#pragma unroll
+          for (int u = 0; u < NH; ++u)
+            tc::tma3(sm.q[q] + u * HALF, &p.mq, 64 * u, h * G, s0 + t0 + q * TQ, &sm.q_full[q]);
+        };
+        load_q(0);
+        load(&p.mk, 0);
+        if (nq > 1) load_q(1);
+        load(&p.mv, 0);
+        for (int i = 1; i < n && ok; ++i) {
+          load(&p.mk, KT * i);
+          if (ok) load(&p.mv, KT * i);
+        }
+        if (*abort) {  // given up: let the copies in flight land before the CTA's memory goes
+          for (int q = 0; q < nq; ++q) (void)mbar_wait(&sm.q_full[q], 0);
+          for (int s = max(0, c - STAGES); s < c; ++s) (void)mbar_wait(&sm.kv_full[s % STAGES], (s / STAGES) & 1);
+        }
+      }
+      __syncwarp();
+    } else {
+      // ---- V tiles with masked places: rows past the sequence and non-finite values to 0
+      for (int i = i_mask; i < n; ++i) {
+        const int cv = 2 * i + 1, s = cv % STAGES;
+        // the MMA warp says when the stage holds this tile: these warps see
+        // only some of a stage's phases, so its parity alone could be an older one's
+        if (!tc::wait_warp(&sm.v_go, (i - i_mask) & 1, abort)) break;
+        if (!tc::wait_warp(&sm.kv_full[s], (cv / STAGES) & 1, abort)) break;
+        uint32_t found = 0u;
+        for (int u = (warp - 10) * 32 + lane; u < KT * D / 8; u += 64) {
+          const int key = KT * i + ((u >> 3) & (KT - 1));
+          uint4* at = reinterpret_cast<uint4*>(sm.kv[s]) + u;
+          uint4 x = *at;
+          if (key >= len) {
+            *at = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            const uint4 e = make_uint4(nonfinite2<BF16>(x.x), nonfinite2<BF16>(x.y), nonfinite2<BF16>(x.z),
+                                       nonfinite2<BF16>(x.w));
+            if (e.x | e.y | e.z | e.w) {
+              found = 1u;
+              *at = make_uint4(x.x & ~e.x, x.y & ~e.y, x.z & ~e.z, x.w & ~e.w);
+            }
+          }
+        }
+        if (found) sm.bad_v = 1u;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::arrive(&sm.v_clean);
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 8) tc::tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && sm.abort) set_err(p.err, HX_DEV_ERR_TIMEOUT);
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+// (T, heads, D) rows of 16-bit elements; the box is 64 elements x heads x tokens
+bool make_map(CUtensorMap* m, bool bf16, const void* base, int D, int heads, int64_t T, int64_t sh, int64_t st,
+              int box_heads, int box_tokens) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T};
+  const cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, one[3] = {1, 1, 1};
+  return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+            dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16>
+int launch(const Params& p, int64_t grid, cudaStream_t s) {
+  constexpr int smem = (int)sizeof(Smem<D>) + 1024;
+  static_assert(smem <= 232448, "a CTA has 227 KB of shared memory");
+  if (cudaFuncSetAttribute(prompt_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return HX_ERR_LAUNCH;
+  }
+  prompt_kernel<D, BF16><<<(unsigned)grid, NTHREADS, smem, s>>>(p);
+  HX_LAUNCH_CHECK();
+  return HX_OK;
+}
+
+}  // namespace pr
+}  // namespace hx
+
+using namespace hx;
+
+extern "C" {
+
+HX_API int hx_prompt_attn(void* stream, int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                          const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                          int64_t v_token_stride, int64_t v_head_stride, const int32_t* query_start, int32_t B,
+                          int32_t T, int32_t H, int32_t group, int32_t D, float softmax_scale, void* out, float* lse,
+                          uint32_t* dev_err) {
+  if (B < 0 || T < 0 || H < 1 || group < 1) return HX_ERR_ARG;
+  if (!(softmax_scale > 0.0f) || softmax_scale > 3.0e38f) return HX_ERR_ARG;
+  if (dtype != 1 && dtype != 2) return HX_ERR_UNSUPPORTED;
+  if ((D != 64 && D != 128) || group > pr::ROWS) return HX_ERR_UNSUPPORTED;
+  if (B == 0 || T == 0) return HX_OK;
+  if (!q || !k || !v || !query_start || !out) return HX_ERR_ARG;
+  const int64_t strides[6] = {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
+                              v_head_stride};
+  for (int64_t s : strides)
+    if (s < D || s % 8 || s >= (1ll << 38)) return HX_ERR_ARG;
+  for (const void* x : {q, k, v, (const void*)out})
+    if (reinterpret_cast<uintptr_t>(x) % 16) return HX_ERR_ARG;
+  pr::Params p;
+  const bool bf = dtype == 2;
+  p.TQ = pr::ROWS / group;
+  if (!pr::make_map(&p.mq, bf, q, D, H * group, T, q_head_stride, q_token_stride, group, p.TQ) ||
+      !pr::make_map(&p.mk, bf, k, D, H, T, k_head_stride, k_token_stride, 1, pr::KT) ||
+      !pr::make_map(&p.mv, bf, v, D, H, T, v_head_stride, v_token_stride, 1, pr::KT))
+    return HX_ERR_LAUNCH;
+  p.start = query_start;
+  p.B = B;
+  p.T = T;
+  p.H = H;
+  p.G = group;
+  p.c = softmax_scale * pr::kLog2e;
+  p.v = reinterpret_cast<const uint16_t*>(v);
+  p.v_st = v_token_stride;
+  p.v_sh = v_head_stride;
+  p.out = reinterpret_cast<uint16_t*>(out);
+  p.lse = lse;
+  p.err = dev_err;
+  const int64_t grid = ((int64_t)T / (2 * p.TQ) + B) * H;
+  if (grid > 0x7fffffffll) return HX_ERR_UNSUPPORTED;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (D == 128) return bf ? pr::launch<128, true>(p, grid, s) : pr::launch<128, false>(p, grid, s);
+  return bf ? pr::launch<64, true>(p, grid, s) : pr::launch<64, false>(p, grid, s);
+}
+
+}  // extern "C"

@@ -11,6 +11,8 @@ fp16 staging buffer (src/kvquant/compact_backend.py:225-299):
                  as packed codes, dequantised on chip and attended; returns
                  normalised o (fp32) and lse (natural log)
   selected_lists the selection as ascending page lists (API / tests)
+  prefill        causal attention of prompt chunks, read from the pool
+  prompt_attention  causal attention of whole prompts from their own K and V
 
 quest_select also returns, per (b, h), how many pages each slice of the
 sequence contributes (the threshold kernel's blocks count them as they go),
@@ -336,6 +338,79 @@ def prefill(pool: CompactKVPool, layer_idx: int, query: torch.Tensor, query_star
              ptr(q), ptr(qs), B, Hq // H, scale, ptr(bt), bt.shape[1], ptr(sl), int(max_query_len),
              hxlib.VPOS_PHYSICAL if v_pos == "physical" else 0, ptr(out), ptr(out32), ptr(lse),
              ptr(hxlib.err_word(dev)))
+    return out, lse
+
+
+_PROMPT_DT = {torch.float16: 1, torch.bfloat16: 2}
+
+
+def _rows(t: torch.Tensor):
+    """A (T, heads, D) tensor and its token and head strides as hx_prompt_attn
+    takes them; a copy where the layout does not fit (16-byte rows)."""
+    T, n, D = t.shape
+    st, sh, sd = t.stride()
+    if sd != 1 or t.data_ptr() % 16 or (T > 1 and (st < D or st % 8)) or (n > 1 and (sh < D or sh % 8)):
+        t = t.contiguous()
+        st, sh, _ = t.stride()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t, (st if T > 1 else n * D), (sh if n > 1 else D)
+
+
+def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, query_start: torch.Tensor, *,
+                     softmax_scale: float | None = None, out: torch.Tensor | None = None,
+                     lse: torch.Tensor | None = None):
+    """Causal attention over whole prompts at full precision (one kernel).
+
+    query (T, Hq, D), key and value (T, H, D), fp16 or bf16, D 64 or 128, Hq =
+    group * H: B prompts back to back, prompt b's tokens are rows
+    query_start[b] .. query_start[b + 1] - 1 (query_start (B + 1,) int32 on the
+    device, as paging.extend_tables makes it). Each token attends to its
+    prompt's tokens up to itself. The three may be slices of one projection
+    (last dimension contiguous, strides of 16 bytes; other layouts are
+    copied). Returns (out (T, Hq, D) in the input type, lse (T, Hq) fp32 natural
+    log); rows past the last prompt are not written. ``prefill`` is the same
+    attention read back from the pool's quantised pages; here the prompt's own
+    K and V, before write_kv packs them, give the unquantised result. K and V
+    are read as they are (infinities and NaN of tokens that a row does not see
+    do not reach it). Reference: FlashAttention over vLLM's fp16 cache
+    (src/kvquant/compact_backend.py:194-205).
+    """
+    if query.dim() != 3 or key.dim() != 3 or value.shape != key.shape:
+        raise ValueError(f"expected (T, Hq, D), (T, H, D), (T, H, D), got {tuple(query.shape)}, {tuple(key.shape)}, "
+                         f"{tuple(value.shape)}")
+    T, Hq, D = query.shape
+    H = key.shape[1]
+    if key.shape[0] != T or key.shape[2] != D:
+        raise ValueError(f"query {tuple(query.shape)} and key {tuple(key.shape)} differ in tokens or head size")
+    if query.dtype not in _PROMPT_DT or key.dtype != query.dtype or value.dtype != query.dtype:
+        raise TypeError(f"query, key and value must all be float16 or all bfloat16, got {query.dtype}, {key.dtype}, "
+                        f"{value.dtype}")
+    if H < 1 or Hq < 1 or Hq % H:
+        raise ValueError("query heads must be a multiple of KV heads")
+    if query_start.dim() != 1 or query_start.numel() < 1:
+        raise ValueError("query_start should be (B + 1,)")
+    hxlib.require_cuda(query, key, value, query_start, out, lse)
+    dev = query.device
+    if key.device != dev or value.device != dev:
+        raise ValueError("query, key and value must be on one device")
+    scale = float(softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D))
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=query.dtype, device=dev)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous() \
+            or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous {tuple(query.shape)} {query.dtype} tensor on {dev}")
+    if lse is None:
+        lse = torch.empty((T, Hq), dtype=torch.float32, device=dev)
+    elif lse.shape != (T, Hq) or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
+        raise ValueError(f"lse must be a contiguous {(T, Hq)} float32 tensor on {dev}")
+    qs = _i32(query_start, dev)
+    q, qt, qh = _rows(query)
+    k, kt, kh = _rows(key)
+    v, vt, vh = _rows(value)
+    with torch.cuda.device(dev):
+        call("hx_prompt_attn", stream(dev), _PROMPT_DT[query.dtype], ptr(q), qt, qh, ptr(k), kt, kh, ptr(v), vt, vh,
+             ptr(qs), qs.numel() - 1, T, H, Hq // H, D, scale, ptr(out), ptr(lse), ptr(hxlib.err_word(dev)))
     return out, lse
 
 

@@ -451,6 +451,29 @@ HX_API int hx_prefill_attn(void* stream, const hx_pool_layer* pool, const hx_lay
                            uint16_t* out16, float* out32, float* lse, uint32_t* dev_err);
 
 /*
+ * Causal attention over whole prompts at full precision (no pool): B sequences
+ * back to back, sequence b's tokens are rows query_start[b] .. query_start[b+1]
+ * - 1 of T (query_start (B+1) int32, device, ascending). q (T, H*group, D), k
+ * and v (T, H, D) of dtype 1 fp16 or 2 bf16, D 64 or 128, group 1..128; token
+ * and head strides in elements (at least D, multiples of 8; the last dimension
+ * contiguous; base pointers 16-byte aligned), so q, k and v may be slices of
+ * one projection. Query head i reads KV head i / group; token i attends to
+ * tokens 0 .. i of its sequence. Writes out (T, H*group, D) contiguous, in the
+ * input type, and lse (T, H*group) fp32 natural log when non-NULL; rows
+ * outside every sequence keep their contents. K and V of masked places are not
+ * read as numbers: infinities and NaN there change no result. softmax_scale
+ * must be positive. Scores, softmax statistics and the output sum are fp32,
+ * the probabilities enter the second product in the input type. One kernel.
+ * Reference counterpart: vLLM's flash_attn_varlen_func on the prompt
+ * (src/kvquant/compact_backend.py:194-205).
+ */
+HX_API int hx_prompt_attn(void* stream, int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                          const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                          int64_t v_token_stride, int64_t v_head_stride, const int32_t* query_start, int32_t B,
+                          int32_t T, int32_t H, int32_t group, int32_t D, float softmax_scale, void* out, float* lse,
+                          uint32_t* dev_err);
+
+/*
  * hx_decode_attn without a caller scratch buffer: no counterpart in the
  * reference. Its scratch is a fixed array inside this library (64 KB of split
  * counters + 1024 split partials, about 4.3 MB per GPU that loads the
