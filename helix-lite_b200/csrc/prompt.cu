@@ -25,6 +25,7 @@
 // sequence's end and non-finite values by 0 before the product, and rows
 // allowed to see a non-finite value get it added at the end (P > 0 there).
 #include "tcgen.cuh"
+#include "tmap.cuh"
 
 namespace hx {
 namespace pr {
@@ -387,35 +388,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
   if (threadIdx.x == 0 && sm.abort) set_err(p.err, HX_DEV_ERR_TIMEOUT);
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
-        r != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<EncodeFn>(f);
-  }();
-  return fn;
-}
-
-// (T, heads, D) rows of 16-bit elements; the box is 64 elements x heads x tokens
-bool make_map(CUtensorMap* m, bool bf16, const void* base, int D, int heads, int64_t T, int64_t sh, int64_t st,
-              int box_heads, int box_tokens) {
-  EncodeFn fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T};
-  const cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)st * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, one[3] = {1, 1, 1};
-  return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
-            dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, bool BF16>
 int launch(const Params& p, int64_t grid, cudaStream_t s) {
   constexpr int smem = (int)sizeof(Smem<D>) + 1024;
@@ -456,9 +428,9 @@ HX_API int hx_prompt_attn(void* stream, int32_t dtype, const void* q, int64_t q_
   pr::Params p;
   const bool bf = dtype == 2;
   p.TQ = pr::ROWS / group;
-  if (!pr::make_map(&p.mq, bf, q, D, H * group, T, q_head_stride, q_token_stride, group, p.TQ) ||
-      !pr::make_map(&p.mk, bf, k, D, H, T, k_head_stride, k_token_stride, 1, pr::KT) ||
-      !pr::make_map(&p.mv, bf, v, D, H, T, v_head_stride, v_token_stride, 1, pr::KT))
+  if (!make_tmap3(&p.mq, bf, q, D, H * group, T, q_head_stride, q_token_stride, group, p.TQ) ||
+      !make_tmap3(&p.mk, bf, k, D, H, T, k_head_stride, k_token_stride, 1, pr::KT) ||
+      !make_tmap3(&p.mv, bf, v, D, H, T, v_head_stride, v_token_stride, 1, pr::KT))
     return HX_ERR_LAUNCH;
   p.start = query_start;
   p.B = B;

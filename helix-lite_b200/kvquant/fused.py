@@ -12,6 +12,7 @@ fp16 staging buffer (src/kvquant/compact_backend.py:225-299):
                  normalised o (fp32) and lse (natural log)
   selected_lists the selection as ascending page lists (API / tests)
   prefill        causal attention of prompt chunks, read from the pool
+  shared_prefix_decode  decode of a batch on one prefix, read once for all
   prompt_attention  causal attention of whole prompts from their own K and V
 
 quest_select also returns, per (b, h), how many pages each slice of the
@@ -337,6 +338,67 @@ def prefill(pool: CompactKVPool, layer_idx: int, query: torch.Tensor, query_star
         call("hx_prefill_attn", stream(dev), ctypes_ref(pool.layers[layer_idx].struct), ctypes_ref(st_scales),
              ptr(q), ptr(qs), B, Hq // H, scale, ptr(bt), bt.shape[1], ptr(sl), int(max_query_len),
              hxlib.VPOS_PHYSICAL if v_pos == "physical" else 0, ptr(out), ptr(out32), ptr(lse),
+             ptr(hxlib.err_word(dev)))
+    return out, lse
+
+
+def shared_prefix_decode(pool: CompactKVPool, layer_idx: int, query: torch.Tensor, block_table: torch.Tensor,
+                         seq_lens: torch.Tensor, prefix_len: int, *, softmax_scale: float | None = None,
+                         v_pos: str = "logical", n_splits: int | None = None, out: torch.Tensor | None = None,
+                         lse: torch.Tensor | None = None):
+    """Decode attention of a batch whose sequences share a prefix (two kernels).
+
+    query (B, Hq, 128) fp16, one token per sequence; block_table (B, max_pages)
+    and seq_lens (B,) as for ``decode``, with the first prefix_len / 16 entries
+    of every row naming the same pool pages (read from row 0). ``prefix_len`` is
+    a host number of tokens, a multiple of the page size. The prefix's pages
+    are read and dequantised once for the whole batch and meet all its query
+    rows in matrix products on the tensor cores; each sequence's own pages
+    follow, and the parts are joined by their (maximum, sum). Every page is
+    attended (no Quest selection): the result is ``decode`` without a
+    selection, at about the cost of one sequence's prefix. A sequence of
+    length 0 is a padding row (out 0, lse -inf). Returns (out (B, Hq, D) fp16,
+    lse (B, Hq) fp32 natural log).
+    """
+    dev = pool.device
+    if query.dim() != 3:
+        raise ValueError(f"query should be (B, Hq, D), got {tuple(query.shape)}")
+    if v_pos not in ("logical", "physical"):
+        raise ValueError("v_pos must be 'logical' or 'physical'")
+    q = query.to(device=dev, dtype=torch.float16).contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    B, Hq, D = q.shape
+    H, S = pool.num_kv_heads, pool.block_size
+    if Hq % H or Hq == 0:
+        raise ValueError("query heads must be a multiple of KV heads")
+    if block_table.dim() != 2 or block_table.shape[0] < B or seq_lens.shape != (B,):
+        raise ValueError(f"block_table {tuple(block_table.shape)} and seq_lens {tuple(seq_lens.shape)} should have a row "
+                         f"for each of {B} sequences")
+    prefix_len = int(prefix_len)
+    if prefix_len < 0 or prefix_len % S or prefix_len // S > block_table.shape[1]:
+        raise ValueError(f"prefix_len must be a multiple of {S} within the block table, got {prefix_len}")
+    bt = _i32(block_table, dev)
+    sl = _i32(seq_lens, dev)
+    scale = float(softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D))
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=torch.float16, device=dev)
+    elif out.shape != q.shape or out.dtype != torch.float16 or out.device != q.device or not out.is_contiguous() \
+            or out.data_ptr() % 8:
+        raise ValueError(f"out must be a contiguous {tuple(q.shape)} float16 tensor on {dev}")
+    if lse is None:
+        lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+    elif lse.shape != (B, Hq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        raise ValueError(f"lse must be a contiguous {(B, Hq)} float32 tensor on {dev}")
+    L = hxlib.lib()
+    ns = int(n_splits) if n_splits is not None else L.hx_prefix_splits(B, H, Hq // H, prefix_len // S)
+    # from torch's allocator, so calls on different streams or in different captured graphs never share it
+    scr = torch.empty((max(16, L.hx_prefix_scratch_bytes(B, H, Hq // H, ns)),), dtype=torch.uint8, device=dev)
+    st_scales, _keep = pool.scales.device_layer(layer_idx, dev)
+    with torch.cuda.device(dev):
+        call("hx_prefix_decode", stream(dev), ctypes_ref(pool.layers[layer_idx].struct), ctypes_ref(st_scales), ptr(q), B,
+             Hq // H, scale, ptr(bt), bt.shape[1], ptr(sl), prefix_len // S,
+             hxlib.VPOS_PHYSICAL if v_pos == "physical" else 0, ns, ptr(scr), ptr(out), ptr(lse),
              ptr(hxlib.err_word(dev)))
     return out, lse
 

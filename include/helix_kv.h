@@ -474,6 +474,32 @@ HX_API int hx_prompt_attn(void* stream, int32_t dtype, const void* q, int64_t q_
                           uint32_t* dev_err);
 
 /*
+ * One decode token per sequence of a batch whose sequences share their first
+ * prefix_pages pool pages: the prefix is read and dequantised once for all of
+ * them. q (B, H*group, D) fp16 contiguous (group <= 128, D = 128, page size 16);
+ * block_table (B rows of bt_stride entries) holds each sequence's whole table,
+ * of which the first prefix_pages entries are read from row 0 only; seq_lens[b]
+ * counts all tokens and is at least 16 * prefix_pages, or 0 for a padding row
+ * (out 0, lse -inf); a shorter one is HX_DEV_ERR_BOUNDS and its row as for
+ * padding. All pages are attended (no selection). V rows by the logical
+ * position, or the physical one with HX_VPOS_PHYSICAL in flags. n_splits: CTAs
+ * along the prefix per (KV head, block of query rows), hx_prefix_splits() or any
+ * number up to ceil(prefix_pages / 8), 0 if and only if prefix_pages is 0.
+ * scratch: hx_prefix_scratch_bytes bytes, 16-byte aligned, no initial contents;
+ * calls that may overlap need their own. Writes out (B, H*group, D) fp16 and
+ * lse (B, H*group) natural log when non-NULL. softmax_scale must be positive.
+ * Scores, statistics and sums are fp32; the probabilities enter the second
+ * product as fp16. Two kernels. No reference counterpart (the reference decodes
+ * one sequence, src/kvquant/compact_backend.py:194-299).
+ */
+HX_API int32_t hx_prefix_splits(int32_t B, int32_t H, int32_t group, int32_t prefix_pages);
+HX_API int64_t hx_prefix_scratch_bytes(int32_t B, int32_t H, int32_t group, int32_t n_splits);
+HX_API int hx_prefix_decode(void* stream, const hx_pool_layer* pool, const hx_layer_scales* sc, const uint16_t* q,
+                            int32_t B, int32_t group, float softmax_scale, const int32_t* block_table,
+                            int32_t bt_stride, const int32_t* seq_lens, int32_t prefix_pages, int32_t flags,
+                            int32_t n_splits, void* scratch, uint16_t* out, float* lse, uint32_t* dev_err);
+
+/*
  * hx_decode_attn without a caller scratch buffer: no counterpart in the
  * reference. Its scratch is a fixed array inside this library (64 KB of split
  * counters + 1024 split partials, about 4.3 MB per GPU that loads the
