@@ -5,21 +5,23 @@
 //   first prefix_len tokens being the same pool pages for every sequence
 //
 // The query rows of a KV head (sequences x heads of the group) are the M side
-// of a matrix product over each dequantised tile of 128 tokens (8 pages). Work
-// items, one a CTA:
-//   prefix  (KV head, block of two 128-row query tiles, split of the prefix):
-//           both tiles use each dequantised key tile. A block with one tile
-//           only runs it twice, on the even and on the odd key tiles
-//   suffix  (KV head, sequence): the sequence's own pages, its G rows alone,
-//           again as two streams of key tiles
+// of a matrix product over each dequantised tile of 128 tokens (8 pages). A
+// CTA (one an SM) takes work items of one KV head, one after another:
+//   prefix  (block of two 128-row query tiles, split of the prefix): both tiles
+//           use each dequantised key tile. A block with one tile only runs it
+//           twice, on the even and on the odd key tiles
+//   suffix  (sequence): the sequence's own pages, its G rows alone, again as two
+//           streams of key tiles
 // Each leaves unnormalised partials (m, l, O) per row; a second kernel joins a
-// row's partials. Roles in a CTA (20 warps):
+// row's partials. Roles in a CTA (25 warps):
 //   0-7    two softmax warpgroups, a row a thread (as in the prompt kernel: S
 //          and P in TMEM, the maximum moves only past 2^8)
-//   8-15   dequantisation: warp w turns page w of each tile into 16 rows of the
-//          swizzled K and V operands (level tables by prmt-built addresses,
-//          registers for nuq4 V past t_cal), outliers patched in
-//   16     the matrix products (tcgen05.mma, one thread); 17 the query tiles
+//   8-15   K dequantisation: warp w turns page w of each tile into 16 rows of the
+//          swizzled operand (per-channel level tables in shared memory, one
+//          prmt-built address a code), outliers patched in
+//   16-23  V dequantisation likewise: levels picked out of registers by prmt
+//          (each token's own row before t_cal, the last row after it)
+//   24     the query tiles and the matrix products (tcgen05.mma, one thread)
 #include "dequant.cuh"
 #include "tcgen.cuh"
 #include "tmap.cuh"
@@ -29,7 +31,7 @@ namespace px {
 
 constexpr int D = 128, S = 16, KT = 128, ROWS = 128, PAGES = KT / S;
 constexpr int STAGES = 4;
-constexpr int NTHREADS = 640;
+constexpr int NTHREADS = 800;  // 25 warps: 72 registers a thread
 constexpr int HALF = KT * 128;  // bytes of 128 rows of 64 fp16
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;
@@ -38,9 +40,9 @@ struct Smem {
   alignas(1024) uint8_t q[2][ROWS * D * 2];
   alignas(1024) uint8_t kv[STAGES][KT * D * 2];
   alignas(256) uint16_t klut[16 * D + 128];      // K tables, bank-spread (32 bytes of room after every 32 channels)
-  alignas(256) uint16_t vlut[PAGES][S * 16];     // V levels per token of each warp's page (before t_cal)
   alignas(256) uint32_t vpair[16];               // nuq2 V past t_cal: level pairs by code pair
   alignas(16) uint32_t vplane[8];                // nuq4 V past t_cal: byte planes
+  alignas(16) uint8_t codes[2][PAGES][1024];     // each producer warp's next page (K, V)
   uint64_t q_full[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], drain;
   uint32_t tmem, abort;
 };
@@ -49,7 +51,7 @@ struct Params {
   CUtensorMap mq;
   hx_pool_layer pool;
   hx_layer_scales sc;
-  int B, G, TQ, RB;          // sequences, heads of a group, sequences a tile, row blocks
+  int B, G, TQ, RB, J;       // sequences, heads of a group, sequences a tile, row blocks, CTAs a head
   float c;                   // softmax scale * log2 e
   const int32_t* bt;
   int bt_stride;
@@ -66,45 +68,259 @@ HX_DEVINL uint32_t pack_h2(float lo, float hi) {
   return r;
 }
 
+// A CTA's items: its split of the prefix, then the suffixes of sequences j, j +
+// J, ... (j the CTA's place among the J of its head). Every role walks them alike.
+struct Item {
+  int seq0, page0, pages, tokens, pidx, n;  // first sequence of the rows; pages [page0, page0 + pages) of table row trow
+  int64_t trow;
+  bool two, suffix;                         // two query tiles (else one tile, two streams of key tiles)
+};
+
+HX_DEVINL bool get_item(const Params& p, int j, int idx, Item& it) {
+  const int lead = p.n_splits > 0 ? 1 : 0;
+  if (idx < lead) {
+    const int rb = j % p.RB, split = j / p.RB;
+    it.suffix = false;
+    it.seq0 = rb * 2 * p.TQ;
+    it.two = it.seq0 + p.TQ < p.B;
+    const int nt = (p.prefix_pages + PAGES - 1) / PAGES;
+    const int ta = (int)((int64_t)nt * split / p.n_splits), te = (int)((int64_t)nt * (split + 1) / p.n_splits);
+    it.page0 = ta * PAGES;
+    it.pages = min(te * PAGES, p.prefix_pages) - it.page0;
+    it.tokens = it.pages * S;
+    it.pidx = 2 * split;
+    it.trow = 0;
+  } else {
+    const int b = j + (idx - lead) * p.J;
+    if (b >= p.B) return false;
+    const int len = p.seq_lens[b];
+    it.suffix = true;
+    it.two = false;
+    it.seq0 = b;
+    it.page0 = p.prefix_pages;
+    it.tokens = len - p.prefix_pages * S;
+    if (it.tokens < 0 || (len - 1) / S >= p.bt_stride) it.tokens = 0;  // the merge flags a bad length
+    it.pages = (it.tokens + S - 1) / S;
+    it.pidx = 2 * p.n_splits;
+    it.trow = (int64_t)b * p.bt_stride;
+  }
+  it.n = (it.pages + PAGES - 1) / PAGES;
+  return true;
+}
+
+// entry (token << 24 | channel << 16 | value) into the page's rows
+HX_DEVINL void patch(uint32_t slab, uint32_t e, int valid, uint32_t* err) {
+  const uint32_t tt = e >> 24, d = (e >> 16) & 0xFFu;
+  if (tt >= (uint32_t)S || d >= (uint32_t)D) {
+    set_err(err, HX_DEV_ERR_BOUNDS);
+  } else if ((int)tt < valid) {
+    const uint32_t off = (d >> 6) * HALF + tt * 128 + ((((d >> 3) & 7) ^ (tt & 7)) << 4) + (d & 7) * 2;
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(slab + off), "h"((uint16_t)(e & 0xFFFFu)) : "memory");
+  }
+}
+
+// 16 levels for 16 2-bit codes from a 4-entry table held as byte planes (low, high) in registers
+HX_DEVINL void crumbs_reg(uint32_t w, uint32_t lb, uint32_t hb, uint4& o0, uint4& o1) {
+  const uint32_t e = w & 0x33333333u, d = (w >> 2) & 0x33333333u;  // codes 0, 2, .. 14 and 1, 3, .. 15 as selectors
+  uint32_t o[8];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const uint32_t es = g ? e >> 16 : e, ds = g ? d >> 16 : d;
+    const uint32_t le = prmt(lb, 0u, es & 0xFFFFu), he = prmt(hb, 0u, es & 0xFFFFu);
+    const uint32_t lo = prmt(lb, 0u, ds & 0xFFFFu), ho = prmt(hb, 0u, ds & 0xFFFFu);
+    const uint32_t e01 = prmt(le, he, 0x5140u), e23 = prmt(le, he, 0x7362u);
+    const uint32_t d01 = prmt(lo, ho, 0x5140u), d23 = prmt(lo, ho, 0x7362u);
+    o[4 * g] = prmt(e01, d01, 0x5410u);
+    o[4 * g + 1] = prmt(e01, d01, 0x7632u);
+    o[4 * g + 2] = prmt(e23, d23, 0x5410u);
+    o[4 * g + 3] = prmt(e23, d23, 0x7632u);
+  }
+  o0 = make_uint4(o[0], o[1], o[2], o[3]);
+  o1 = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+HX_DEVINL void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+HX_DEVINL uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// ---- dequantisation: warp w's page of every tile, K (kv 0) or V (kv 1) operand.
+// A lane has 64 channels of one token. Its codes come a tile ahead by cp.async
+// into its own 32 bytes of shared memory (72 registers a thread do not hold
+// them as well: spilled, the kernel took 1.3 times as long), the page's list
+// record and table entry a tile ahead in registers, none of them looked at
+// before its turn (a look at load time waits for the load: 1.2 times).
+template <int BITS, int KV, int SEG, int BASE>
+HX_DEVINL void produce(const Params& p, Smem& sm, int h, int j, int w) {
+  const int lane = threadIdx.x & 31, t = lane >> 1, half = lane & 1;
+  const int Tc = p.sc.t_cal, NB = p.pool.num_blocks;
+  constexpr int RB = D * BITS / 8, W = BITS * 2, E = BITS == 2 ? 4 : 1;  // row bytes; code words a lane; entries at once
+  const uint8_t* code0 = p.pool.codes + (int64_t)h * NB * SEG + BASE + t * RB + half * (RB / 2);
+  const uint32_t* dir0 = p.pool.dir + ((int64_t)h * NB * 2 + KV) * 4;
+  const uint32_t own = smem_u32(sm.codes[KV][w]) + 16 * lane;  // 16-byte chunk u of the lane's half row at own + 512 u
+  const uint32_t store0 = half * HALF + (16 * w + t) * 128 + 16u * ((4u * half) ^ (t & 7));
+  volatile uint32_t* abort = &sm.abort;
+  constexpr int kNone = -0x7fffffff;  // past the item's pages
+  int g = 0;                          // tiles so far: stage 2 (g & 1) + KV
+  Item it;
+  for (int idx = 0; get_item(p, j, idx, it); ++idx) {
+    const int32_t* bt = p.bt + it.trow + it.page0 + w;
+    const int pages = it.pages - w;
+    auto entry = [&](int i) -> int { return PAGES * i < pages ? bt[PAGES * i] : kNone; };
+    uint32_t off = 0u, cap = 0u, cnt = 0u;
+    int phys = -1;
+    auto load = [&](int e) {  // e: a table entry, itself loaded a tile before
+      phys = e >= 0 && e < NB ? e : -1;
+      if (phys >= 0) {
+        const uint8_t* c = code0 + (int64_t)e * SEG;
+        cp16(own, c);
+        if (BITS == 4) cp16(own + 512, c + 16);
+        const uint4 d = __ldg(reinterpret_cast<const uint4*>(dir0 + (int64_t)e * 8));
+        off = d.x, cap = d.y, cnt = d.z;
+      } else {
+        off = cap = cnt = 0u;
+        if (e != kNone && lane == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int e_next = entry(1);
+    load(entry(0));
+    for (int i = 0; i < it.n; ++i, ++g) {
+      // ---- this page's codes into registers, the next page's on their way
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      uint32_t c[W];
+      // half 1 takes its 16-byte output chunks in the order 4 .. 7, 0 .. 3: the stores of four tokens' halves then
+      // meet eight bank groups
+      if (BITS == 4) {
+        const uint4 x = lds128(own + 512 * half), y = lds128(own + 512 * (half ^ 1));
+        c[0] = x.x, c[1] = x.y, c[2] = x.z, c[3] = x.w;
+        c[W - 4] = y.x, c[W - 3] = y.y, c[W - 2] = y.z, c[W - 1] = y.w;
+      } else {
+        const uint4 x = lds128(own);
+        c[0] = half ? x.z : x.x, c[1] = half ? x.w : x.y, c[2] = half ? x.x : x.z, c[3] = half ? x.y : x.w;
+      }
+      if (cnt > cap || (int64_t)off + cnt > p.pool.arena_capacity) {  // a record that leaves the arena
+        set_err(p.err, HX_DEV_ERR_BOUNDS);
+        cnt = 0u;
+      }
+      const uint32_t* list = p.pool.arena + off + lane;
+      const int left = (int)cnt - lane;  // the lane's entries: list[0], list[32], ... while below left
+      uint32_t ent[E];
+#pragma unroll
+      for (int u = 0; u < E; ++u) ent[u] = 32 * u < left ? __ldg(list + 32 * u) : 0u;
+      const bool here = phys >= 0;
+      // V: the token's own level row, if the page has tokens before the last calibrated position
+      const int64_t pos0 = (int64_t)(p.vphys ? phys : it.page0 + PAGES * i + w) * S;
+      const bool tail = !KV || pos0 >= Tc - 1;
+      constexpr int LW = BITS == 4 ? 8 : 2;
+      uint32_t lev[LW];  // levels 2u, 2u + 1
+      if (KV && here && !tail) {
+        const int L = p.sc.levels_v;
+        const uint16_t* row = p.sc.v_poles + ((int64_t)h * Tc + min(pos0 + t, (int64_t)Tc - 1)) * L;
+        if (L == (1 << BITS) && (reinterpret_cast<uintptr_t>(p.sc.v_poles) & 15u) == 0) {
+          if (BITS == 4) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(row)), y = __ldg(reinterpret_cast<const uint4*>(row) + 1);
+            lev[0] = x.x, lev[1] = x.y, lev[2 % LW] = x.z, lev[3 % LW] = x.w;
+            lev[4 % LW] = y.x, lev[5 % LW] = y.y, lev[6 % LW] = y.z, lev[7 % LW] = y.w;
+          } else {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(row));
+            lev[0] = x.x, lev[1] = x.y;
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < LW; ++u)
+            lev[u] = (2 * u < L ? (uint32_t)row[2 * u] : 0u) | ((2 * u + 1 < L ? (uint32_t)row[2 * u + 1] : 0u) << 16);
+        }
+      }
+      __syncwarp();  // the codes are in registers: their place may be filled again
+      load(e_next);
+      e_next = entry(i + 2);
+      const int valid = KV ? min(S, it.tokens - (PAGES * i + w) * S) : S;  // K past the tokens is masked as a score
+      const int st = 2 * (g & 1) + KV;
+      if (g >= 2 && !tc::wait_warp(&sm.kv_empty[st], ((g >> 1) & 1) ^ 1, abort)) return;
+      const uint32_t base = smem_u32(sm.kv[0]) + st * (KT * D * 2), at = base + store0, slab = base + 16 * w * 128;
+      if (!here) {  // past the item's pages (masked), or a page id out of range (flagged)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sts128(at ^ (16u * u), make_uint4(0u, 0u, 0u, 0u));
+      } else {
+        if (KV == 0) {
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const uint32_t tab = smem_u32(sm.klut) + 2048u * half + 1024u * (half ^ jj);
+            if (BITS == 4) {
+              const uint32_t low = (64u * half + 32u * (half ^ jj)) * 0x01010101u;
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                sts128(at ^ (64u * jj + 16u * u), lut8_nib<32>(c[(4 * jj + u) % W], low, tab, 256u * u));
+            } else {
+              const uint32_t low = 64u * half * 0x01010101u;
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                uint4 o0, o1;
+                lut8_pair<64>(c[2 * jj + u], low, tab, 512u * u, o0, o1);
+                sts128(at ^ (64u * jj + 32u * u), o0);
+                sts128(at ^ (64u * jj + 32u * u + 16u), o1);
+              }
+            }
+          }
+        } else if (BITS == 4) {
+          uint32_t lb[4], hb[4];
+          if (tail) {
+            const uint4 x = lds128(smem_u32(sm.vplane)), y = lds128(smem_u32(sm.vplane + 4));
+            lb[0] = x.x, lb[1] = x.y, lb[2] = x.z, lb[3] = x.w;
+            hb[0] = y.x, hb[1] = y.y, hb[2] = y.z, hb[3] = y.w;
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              lb[u] = prmt(lev[(2 * u) % LW], lev[(2 * u + 1) % LW], 0x6420u);
+              hb[u] = prmt(lev[(2 * u) % LW], lev[(2 * u + 1) % LW], 0x7531u);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) sts128(at ^ (16u * u), lut8_reg(c[u % W], lb, hb));
+        } else {
+          const uint32_t lb = prmt(lev[0], lev[1], 0x6420u), hb = prmt(lev[0], lev[1], 0x7531u);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint4 o0, o1;
+            if (tail) lut8_pair<0>(c[u], 0u, smem_u32(sm.vpair), 0u, o0, o1);
+            else crumbs_reg(c[u], lb, hb, o0, o1);
+            sts128(at ^ (32u * u), o0);
+            sts128(at ^ (32u * u + 16u), o1);
+          }
+        }
+        // rows that are not attended are zeroed: P is 0 there, but 0 * inf is not
+        if (KV && valid < S && t >= valid) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) sts128(at ^ (16u * u), make_uint4(0u, 0u, 0u, 0u));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < E; ++u)
+          if (32 * u < left) patch(slab, ent[u], valid, p.err);
+        for (int e = 32 * E; e < left; e += 32) patch(slab, __ldg(list + e), valid, p.err);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tc::arrive(&sm.kv_full[st]);
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 template <int BK, int BV>
 __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  constexpr int RBK = D * BK / 8, RBV = D * BV / 8, SEG = S * (RBK + RBV);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int H = p.pool.num_kv_heads, G = p.G, TQ = p.TQ, NB = p.pool.num_blocks, Tc = p.sc.t_cal;
+  const int H = p.pool.num_kv_heads, G = p.G, TQ = p.TQ, Tc = p.sc.t_cal;
+  const int h = blockIdx.x % H, j = blockIdx.x / H;
 
-  // ---- the work item
-  const int n_pre = H * p.RB * p.n_splits;
-  const bool suffix = (int)blockIdx.x >= n_pre;
-  const int it = suffix ? (int)blockIdx.x - n_pre : (int)blockIdx.x;
-  const int h = it % H;
-  int seq0, page0, pages, tokens, pidx;  // first sequence of the rows; the item's pages in table row `trow`
-  bool two;                              // two query tiles (else one tile, two streams of key tiles)
-  if (suffix) {
-    seq0 = it / H;
-    const int len = p.seq_lens[seq0], pre = p.prefix_pages * S;
-    tokens = len - pre;
-    if (tokens <= 0 || (len - 1) / S >= p.bt_stride) return;  // the merge flags a bad length
-    page0 = p.prefix_pages;
-    pages = (tokens + S - 1) / S;
-    two = false;
-    pidx = 2 * p.n_splits;
-  } else {
-    const int rb = (it / H) % p.RB, split = it / H / p.RB;
-    seq0 = rb * 2 * TQ;
-    two = seq0 + TQ < p.B;
-    const int nt = (p.prefix_pages + PAGES - 1) / PAGES;
-    const int ta = (int)((int64_t)nt * split / p.n_splits), te = (int)((int64_t)nt * (split + 1) / p.n_splits);
-    page0 = ta * PAGES;
-    pages = min(te * PAGES, p.prefix_pages) - page0;
-    tokens = pages * S;
-    pidx = 2 * split;
-  }
-  const int64_t trow = suffix ? (int64_t)seq0 * p.bt_stride : 0;
-  const int n = (pages + PAGES - 1) / PAGES;  // key tiles
-
-  if (warp == 16) {
+  if (warp == 24) {
     if (lane == 0) {
       for (int q = 0; q < 2; ++q) {
         mbar_init(&sm.q_full[q], 1);
@@ -152,417 +368,250 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
   tc::fence_after();
   const uint32_t tmem = sm.tmem;
   volatile uint32_t* abort = &sm.abort;
+  Item it;
 
   if (warp < 8) {
     // ---- softmax: warpgroup q; with two tiles q is the tile, else the stream of key tiles q, q + 2, ...
-    tc::regs_inc<120>();
     const int q = warp >> 2, r = threadIdx.x & 127;
-    const int seq = seq0 + (two ? q * TQ : 0) + r / G;
-    const bool live = suffix ? r < G : (r < TQ * G && seq < p.B);
-    const bool any = __any_sync(0xffffffffu, live);  // warps without rows only keep step
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t sb = tmem + lanes + 128 * q, ob = tmem + lanes + 256 + 128 * q;
-    const int first = two ? 0 : q, step = two ? 1 : 2;
-    float m = -INFINITY, l = 0.0f;
+    int used = 0, done = 0;  // S tiles and O results of this warpgroup so far
     bool ok = true;
-    int k = 0;
-    for (int i = first; i < n && ok; i += step, ++k) {
-      ok = tc::wait_warp(&sm.s_full[q], k & 1, abort);
-      if (!ok) break;
-      if (any) {
-        tc::fence_after();
-        const int lim = tokens - KT * i;  // valid keys of the tile
-        uint32_t s[64];
-        float mt = -INFINITY;
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          tc::ld32(s, sb + 64 * hf);
-          tc::ld32(s + 32, sb + 64 * hf + 32);
-          tc::wait_ld();
-          if (lim < KT) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) s[j] = 64 * hf + j < lim ? s[j] : 0xff800000u;
-          }
+    for (int idx = 0; ok && get_item(p, j, idx, it); ++idx) {
+      const int seq = it.seq0 + (it.two ? q * TQ : 0) + r / G;
+      const bool live = it.suffix ? r < G : (r < TQ * G && seq < p.B);
+      const bool any = __any_sync(0xffffffffu, live);  // warps without rows only keep step
+      const int first = it.two ? 0 : q, step = it.two ? 1 : 2;
+      float m = -INFINITY, l = 0.0f;
+      int k = 0;
+      for (int i = first; i < it.n && ok; i += step, ++k, ++used) {
+        ok = tc::wait_warp(&sm.s_full[q], used & 1, abort);
+        if (!ok) break;
+        if (any) {
+          tc::fence_after();
+          const int lim = it.tokens - KT * i;  // valid keys of the tile
           float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-          for (int j = 0; j < 64; j += 4) {
-            mx[0] = fmaxf(mx[0], fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
-            mx[1] = fmaxf(mx[1], fmaxf(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])));
-          }
-          mt = fmaxf(mt, fmaxf(mx[0], mx[1]));
-        }
-        const bool move = (mt - m) * p.c > kSlack;
-        if (__any_sync(0xffffffffu, move)) {
-          const float mn = move ? mt : m;
-          const float a = move ? tc::ex2((m - mn) * p.c) : 1.0f;
-          m = mn;
-          l *= a;
-          if (k > 0) {  // the stream's O is complete: this S was issued after it
-            const uint64_t a2 = tc::f2_pack(a, a);
 #pragma unroll 1
-            for (int u = 0; u < D / 32; ++u) {
-              uint32_t o[32];
-              tc::ld32(o, ob + 32 * u);
-              tc::wait_ld();
+          for (int qt = 0; qt < 4; ++qt) {
+            uint32_t s[32];
+            tc::ld32(s, sb + 32 * qt);
+            tc::wait_ld();
+            if (lim < KT) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                float x, y;
-                tc::f2_unpack(tc::f2_mul(tc::f2_pack(__uint_as_float(o[j]), __uint_as_float(o[j + 1])), a2), x, y);
-                o[j] = __float_as_uint(x);
-                o[j + 1] = __float_as_uint(y);
+              for (int c = 0; c < 32; ++c) s[c] = 32 * qt + c < lim ? s[c] : 0xff800000u;
+            }
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              mx[0] = fmaxf(mx[0], fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
+              mx[1] = fmaxf(mx[1], fmaxf(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])));
+            }
+          }
+          const float mt = fmaxf(mx[0], mx[1]);
+          const bool move = (mt - m) * p.c > kSlack;
+          if (__any_sync(0xffffffffu, move)) {
+            const float mn = move ? mt : m;
+            const float a = move ? tc::ex2((m - mn) * p.c) : 1.0f;
+            m = mn;
+            l *= a;
+            if (k > 0) {  // the stream's O is complete: this S was issued after it
+              const uint64_t a2 = tc::f2_pack(a, a);
+#pragma unroll 1
+              for (int u = 0; u < D / 32; ++u) {
+                uint32_t o[32];
+                tc::ld32(o, ob + 32 * u);
+                tc::wait_ld();
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                  float x, y;
+                  tc::f2_unpack(tc::f2_mul(tc::f2_pack(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), a2), x, y);
+                  o[c] = __float_as_uint(x);
+                  o[c + 1] = __float_as_uint(y);
+                }
+                tc::st32(ob + 32 * u, o);
               }
-              tc::st32(ob + 32 * u, o);
+            }
+          }
+          const float mb = m == -INFINITY ? 0.0f : -m * p.c;
+          const uint64_t c2 = tc::f2_pack(p.c, p.c), mb2 = tc::f2_pack(mb, mb);
+          uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll 1
+          for (int qt = 0; qt < 4; ++qt) {  // P of a quarter overwrites S columns already used
+            uint32_t s[32];
+            tc::ld32(s, sb + 32 * qt);
+            tc::wait_ld();
+            if (lim < KT) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) s[c] = 32 * qt + c < lim ? s[c] : 0xff800000u;
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              float x, y;
+              tc::f2_unpack(tc::f2_fma(tc::f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, mb2), x, y);
+              x = tc::ex2(x);
+              y = tc::ex2(y);
+              sum[(c >> 1) & 1] = tc::f2_add(sum[(c >> 1) & 1], tc::f2_pack(x, y));
+              pk[c >> 1] = pack_h2(x, y);
+            }
+            tc::st16(sb + 16 * qt, pk);
+          }
+          float x, y;
+          tc::f2_unpack(tc::f2_add(sum[0], sum[1]), x, y);
+          l += x + y;
+          tc::wait_st();
+          tc::fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) tc::arrive(&sm.p_full[q]);
+      }
+      if (it.n == 0) continue;
+      // ---- the rows' partials
+      if (ok && k > 0) ok = tc::wait_warp(&sm.o_full[q], done++ & 1, abort);
+      if (ok && any) {
+        tc::fence_after();
+        const int64_t rows = (int64_t)p.B * H * G;
+        const int64_t row = ((int64_t)(it.suffix ? it.seq0 : seq) * H + h) * G + (it.suffix ? r : r % G);
+        const int64_t at = (int64_t)(it.pidx + (it.two ? 0 : q)) * rows + row;
+        if (live) p.part_ml[at] = make_float2(m * p.c, l);
+        if (k > 0) {
+#pragma unroll 1
+          for (int u = 0; u < D / 32; ++u) {
+            uint32_t o[32];
+            tc::ld32(o, ob + 32 * u);
+            tc::wait_ld();
+            if (live) {
+              uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + 32 * u);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) dst[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
             }
           }
         }
-        const float mb = m == -INFINITY ? 0.0f : -m * p.c;
-        const uint64_t c2 = tc::f2_pack(p.c, p.c), mb2 = tc::f2_pack(mb, mb);
-        uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {  // P of a half overwrites S columns already used
-          tc::ld32(s, sb + 64 * hf);
-          tc::ld32(s + 32, sb + 64 * hf + 32);
-          tc::wait_ld();
-          if (lim < KT) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) s[j] = 64 * hf + j < lim ? s[j] : 0xff800000u;
-          }
-          uint32_t pk[32];
-#pragma unroll
-          for (int j = 0; j < 64; j += 2) {
-            float x, y;
-            tc::f2_unpack(tc::f2_fma(tc::f2_pack(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), c2, mb2), x, y);
-            x = tc::ex2(x);
-            y = tc::ex2(y);
-            sum[(j >> 1) & 1] = tc::f2_add(sum[(j >> 1) & 1], tc::f2_pack(x, y));
-            pk[j >> 1] = pack_h2(x, y);
-          }
-          tc::st32(sb + 32 * hf, pk);
-        }
-        float x, y;
-        tc::f2_unpack(tc::f2_add(sum[0], sum[1]), x, y);
-        l += x + y;
-        tc::wait_st();
+        // a block of two tiles has one partial per split: the second place stays empty
+        if (it.two && live) p.part_ml[at + rows] = make_float2(-INFINITY, 0.0f);
         tc::fence_before();
       }
       __syncwarp();
-      if (lane == 0) tc::arrive(&sm.p_full[q]);
-    }
-    // ---- the rows' partials
-    if (ok && k > 0) ok = tc::wait_warp(&sm.o_full[q], 0, abort);
-    tc::fence_after();
-    if (ok && any) {
-      const int64_t rows = (int64_t)p.B * H * G;
-      const int64_t row = ((int64_t)(suffix ? seq0 : seq) * H + h) * G + (suffix ? r : r % G);
-      const int64_t at = (int64_t)(pidx + (two ? 0 : q)) * rows + row;
-      if (live) p.part_ml[at] = make_float2(m * p.c, l);
-      if (k > 0) {
-#pragma unroll 1
-        for (int u = 0; u < D / 32; ++u) {
-          uint32_t o[32];
-          tc::ld32(o, ob + 32 * u);
-          tc::wait_ld();
-          if (live) {
-            uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + 32 * u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-          }
-        }
-      }
-      // a block of two tiles has one partial per split: the second place stays empty
-      if (two && live) p.part_ml[at + rows] = make_float2(-INFINITY, 0.0f);
     }
   } else if (warp < 16) {
-    // ---- dequantisation: warp w's page of every tile
-    const int w = warp - 8, t = lane >> 1, half = lane & 1;
-    const uint8_t* codes = p.pool.codes + (int64_t)h * NB * SEG;
-    const uint32_t* dirs = p.pool.dir + (int64_t)h * NB * 8;
-    constexpr int EK = BK == 2 ? 4 : 1, EV = BV == 2 ? 4 : 1;  // outlier entries a lane holds ahead
-    constexpr int WK = BK * 2, WV = BV * 2;                      // code words a lane holds (64 channels)
-    struct Ahead {
-      uint32_t k[WK], v[WV];
-      uint4 dk, dv;
-      int phys;
-    };
-    auto phys_of = [&](int i) -> int {
-      const int pg = PAGES * i + w;
-      if (pg >= pages) return -1;
-      const int pp = p.bt[trow + page0 + pg];
-      if (pp >= 0 && pp < NB) return pp;
-      if (lane == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
-      return -1;
-    };
-    auto load = [&](Ahead& a, int pp) {
-      a.phys = pp;
-      if (pp < 0) {
-        a.dk = a.dv = make_uint4(0u, 0u, 0u, 0u);
-        return;
-      }
-      // half 1 takes its 16-byte chunks in the order 4 .. 7, 0 .. 3: the stores of a row pair then meet 8 bank groups
-      const uint8_t* seg = codes + (int64_t)pp * SEG;
-      const uint8_t* kr = seg + t * RBK + half * (RBK / 2);
-      const uint8_t* vr = seg + S * RBK + t * RBV + half * (RBV / 2);
-      if (BK == 4) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(kr + 16 * half));
-        const uint4 y = __ldg(reinterpret_cast<const uint4*>(kr + 16 * (half ^ 1)));
-        a.k[0] = x.x, a.k[1] = x.y, a.k[2] = x.z, a.k[3] = x.w;
-        a.k[WK - 4] = y.x, a.k[WK - 3] = y.y, a.k[WK - 2] = y.z, a.k[WK - 1] = y.w;
-      } else {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(kr + 8 * half));
-        const uint2 y = __ldg(reinterpret_cast<const uint2*>(kr + 8 * (half ^ 1)));
-        a.k[0] = x.x, a.k[1] = x.y, a.k[2] = y.x, a.k[3] = y.y;
-      }
-      if (BV == 4) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(vr + 16 * half));
-        const uint4 y = __ldg(reinterpret_cast<const uint4*>(vr + 16 * (half ^ 1)));
-        a.v[0] = x.x, a.v[1] = x.y, a.v[2] = x.z, a.v[3] = x.w;
-        a.v[WV - 4] = y.x, a.v[WV - 3] = y.y, a.v[WV - 2] = y.z, a.v[WV - 1] = y.w;
-      } else {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(vr + 8 * half));
-        const uint2 y = __ldg(reinterpret_cast<const uint2*>(vr + 8 * (half ^ 1)));
-        a.v[0] = x.x, a.v[1] = x.y, a.v[2] = y.x, a.v[3] = y.y;
-      }
-      a.dk = __ldg(reinterpret_cast<const uint4*>(dirs + (int64_t)pp * 8));
-      a.dv = __ldg(reinterpret_cast<const uint4*>(dirs + (int64_t)pp * 8 + 4));
-    };
-    auto fits = [&](uint4& d) {  // a record that leaves the arena is flagged and its entries left out
-      if (d.z > d.y || (int64_t)d.x + d.z > p.pool.arena_capacity) {
-        if (lane == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
-        d.z = 0u;
-      }
-    };
-    const uint32_t t7 = t & 7;
-    const uint32_t store0 = half * HALF + (16 * w + t) * 128 + 16u * ((4u * half) ^ t7);
-    // entry -> byte offset in the page's rows: token << 24 | channel << 16 | value
-    auto patch = [&](uint32_t slab, uint32_t e, int valid) {
-      const uint32_t tt = e >> 24, d = (e >> 16) & 0xFFu;
-      if (tt >= (uint32_t)S || d >= (uint32_t)D) {
-        set_err(p.err, HX_DEV_ERR_BOUNDS);
-      } else if ((int)tt < valid) {
-        const uint32_t off = (d >> 6) * HALF + tt * 128 + ((((d >> 3) & 7) ^ (tt & 7)) << 4) + (d & 7) * 2;
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(slab + off), "h"((uint16_t)(e & 0xFFFFu)) : "memory");
-      }
-    };
-    uint32_t lb[4], hb[4];
-    if (BV == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lb[i] = sm.vplane[i], hb[i] = sm.vplane[4 + i];
-    }
-    Ahead cur, nxt;
-    load(cur, phys_of(0));
-    int pp1 = n > 1 ? phys_of(1) : -1;
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      fits(cur.dk);
-      fits(cur.dv);
-      uint32_t ek[EK], ev[EV];
-#pragma unroll
-      for (int u = 0; u < EK; ++u) ek[u] = lane + 32 * u < (int)cur.dk.z ? __ldg(p.pool.arena + cur.dk.x + lane + 32 * u) : ~0u;
-#pragma unroll
-      for (int u = 0; u < EV; ++u) ev[u] = lane + 32 * u < (int)cur.dv.z ? __ldg(p.pool.arena + cur.dv.x + lane + 32 * u) : ~0u;
-      if (i + 1 < n) {
-        load(nxt, pp1);
-        pp1 = i + 2 < n ? phys_of(i + 2) : -1;
-      }
-      const int valid = min(S, tokens - (PAGES * i + w) * S);  // tokens of the page that are attended
-      // ---- K
-      {
-        const int c = 2 * i, s = c % STAGES;
-        if (c >= STAGES) ok = tc::wait_warp(&sm.kv_empty[s], ((c / STAGES) & 1) ^ 1, abort);
-        if (!ok) break;
-        const uint32_t base = smem_u32(sm.kv[s]), at = base + store0, slab = base + 16 * w * 128;
-        if (cur.phys >= 0) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t tab = smem_u32(sm.klut) + 2048u * half + 1024u * (half ^ j);
-            if (BK == 4) {
-              const uint32_t low = (64u * half + 32u * (half ^ j)) * 0x01010101u;
-#pragma unroll
-              for (int u = 0; u < 4; ++u) sts128(at ^ (64u * j + 16u * u), lut8_nib<32>(cur.k[(4 * j + u) % WK], low, tab, 256u * u));
-            } else {
-              const uint32_t low = 64u * half * 0x01010101u;
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                uint4 o0, o1;
-                lut8_pair<64>(cur.k[(2 * j + u) % WK], low, tab, 512u * u, o0, o1);
-                sts128(at ^ (64u * j + 32u * u), o0);
-                sts128(at ^ (64u * j + 32u * u + 16u), o1);
-              }
-            }
-          }
-          __syncwarp();
-#pragma unroll
-          for (int u = 0; u < EK; ++u)
-            if (lane + 32 * u < (int)cur.dk.z) patch(slab, ek[u], S);
-          for (int e = lane + 32 * EK; e < (int)cur.dk.z; e += 32) patch(slab, __ldg(p.pool.arena + cur.dk.x + e), S);
-        } else {  // past the item's pages (masked), or a page id out of range (flagged)
-#pragma unroll
-          for (int u = 0; u < 8; ++u) sts128(at ^ (16u * u), make_uint4(0u, 0u, 0u, 0u));
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) tc::arrive(&sm.kv_full[s]);
-      }
-      // ---- V; rows that are not attended are zeroed (P is 0 there, but 0 * inf is not)
-      {
-        const int c = 2 * i + 1, s = c % STAGES;
-        if (c >= STAGES) ok = tc::wait_warp(&sm.kv_empty[s], ((c / STAGES) & 1) ^ 1, abort);
-        if (!ok) break;
-        const uint32_t base = smem_u32(sm.kv[s]), at = base + store0, slab = base + 16 * w * 128;
-        if (cur.phys >= 0) {
-          const int64_t pos0 = (int64_t)(p.vphys ? cur.phys : page0 + PAGES * i + w) * S;
-          const bool tail = pos0 >= Tc - 1;  // every token of the page reads the last row
-          if (!tail) {
-            const int L = p.sc.levels_v;
-            __syncwarp();  // the tables' last readers are done
-            for (int x = lane; x < S * 16; x += 32) {
-              const int64_t row = min(pos0 + (x >> 4), (int64_t)Tc - 1);
-              sm.vlut[w][x] = (x & 15) < L ? p.sc.v_poles[((int64_t)h * Tc + row) * L + (x & 15)] : (uint16_t)0;
-            }
-            __syncwarp();
-          }
-          const uint32_t vt = smem_u32(sm.vlut[w]) + 256u * (t >> 3), vlow = 32u * t7 * 0x01010101u;
-          const bool mine = t < valid;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if (BV == 4) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                const uint32_t cw = cur.v[(4 * j + u) % WV];
-                uint4 o = tail ? lut8_reg(cw, lb, hb) : lut8_nib<0>(cw, vlow, vt, 0u);
-                if (!mine) o = make_uint4(0u, 0u, 0u, 0u);
-                sts128(at ^ (64u * j + 16u * u), o);
-              }
-            } else {
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const uint32_t cw = cur.v[(2 * j + u) % WV];
-                uint4 o0, o1;
-                if (tail) lut8_pair<0>(cw, 0u, smem_u32(sm.vpair), 0u, o0, o1);
-                else lut16_crumb<0>(cw, vlow, vt, 0u, o0, o1);
-                if (!mine) o0 = o1 = make_uint4(0u, 0u, 0u, 0u);
-                sts128(at ^ (64u * j + 32u * u), o0);
-                sts128(at ^ (64u * j + 32u * u + 16u), o1);
-              }
-            }
-          }
-          __syncwarp();
-#pragma unroll
-          for (int u = 0; u < EV; ++u)
-            if (lane + 32 * u < (int)cur.dv.z) patch(slab, ev[u], valid);
-          for (int e = lane + 32 * EV; e < (int)cur.dv.z; e += 32) patch(slab, __ldg(p.pool.arena + cur.dv.x + e), valid);
-        } else {
-#pragma unroll
-          for (int u = 0; u < 8; ++u) sts128(at ^ (16u * u), make_uint4(0u, 0u, 0u, 0u));
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) tc::arrive(&sm.kv_full[s]);
-      }
-      cur = nxt;
-    }
+    produce<BK, 0, S * D * (BK + BV) / 8, 0>(p, sm, h, j, warp - 8);
+  } else if (warp < 24) {
+    produce<BV, 1, S * D * (BK + BV) / 8, S * D * BK / 8>(p, sm, h, j, warp - 16);
   } else {
-    tc::regs_dec<48>();
-    if (warp == 16) {
-      // ---- matrix products
-      constexpr uint32_t ids = tc::idesc_f16(0, ROWS, KT, 0), idv = tc::idesc_f16(0, ROWS, D, 1);
-      auto qk = [&](int q, int tile, int stage) {
-        const uint32_t qa = smem_u32(sm.q[tile]), ka = smem_u32(sm.kv[stage]);
+    if (warp == 24) {
+    // ---- query tiles and matrix products
+    constexpr uint32_t ids = tc::idesc_f16(0, ROWS, KT, 0), idv = tc::idesc_f16(0, ROWS, D, 1);
+    int qn[2] = {0, 0}, used[2] = {0, 0};  // loads into a query buffer; S tiles of a warpgroup so far
+    auto load_q = [&](int buf, int seq0) {  // the buffer's last products are complete: their P has been used
+      if (tc::elect()) {
+        mbar_arrive_expect_tx(&sm.q_full[buf], TQ * G * D * 2);
+        for (int u = 0; u < 2; ++u) tc::tma3(sm.q[buf] + u * HALF, &p.mq, 64 * u, h * G, seq0, &sm.q_full[buf]);
+      }
+      ++qn[buf];
+    };
+    auto qk = [&](int q, int buf, int g) {
+      const uint64_t qd = tc::desc128(smem_u32(sm.q[buf]), 0), kd = tc::desc128(smem_u32(sm.kv[2 * (g & 1)]), 0);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k / 4) * HALF + (k % 4) * 32;
-          tc::mma_ss(tmem + 128 * q, tc::desc128(qa + off, 0), tc::desc128(ka + off, 0), ids, k > 0);
-        }
-        tc::commit(&sm.s_full[q]);
-      };
-      auto pv = [&](int q, int stage, bool more) {
-        const uint32_t va = smem_u32(sm.kv[stage]);
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = ((k / 4) * HALF + (k % 4) * 32) >> 4;
+        tc::mma_ss(tmem + 128 * q, qd + off, kd + off, ids, k > 0);
+      }
+      tc::commit(&sm.s_full[q]);
+    };
+    auto pv = [&](int q, int g, bool more) {
+      const uint64_t vd = tc::desc128(smem_u32(sm.kv[2 * (g & 1) + 1]), HALF);
 #pragma unroll
-        for (int k = 0; k < KT / 16; ++k)
-          tc::mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * k, tc::desc128(va + 2048 * k, HALF), idv, more || k > 0);
-      };
-      auto full = [&](int c) { return tc::wait_warp(&sm.kv_full[c % STAGES], (c / STAGES) & 1, abort); };
-      bool ok = tc::wait_warp(&sm.q_full[0], 0, abort);
-      if (two && ok) ok = tc::wait_warp(&sm.q_full[1], 0, abort);
-      if (two) {
-        // tile q of both uses every key tile
-        if (ok) ok = full(0);
-        if (ok && lane == 0) {
+      for (int k = 0; k < KT / 16; ++k)
+        tc::mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * k, vd + 128 * k, idv, more || k > 0);
+    };
+    auto full = [&](int g, int kv) { return tc::wait_warp(&sm.kv_full[2 * (g & 1) + kv], (g >> 1) & 1, abort); };
+    auto p_wait = [&](int q) { return tc::wait_warp(&sm.p_full[q], used[q]++ & 1, abort); };
+    bool ok = true;
+    int g = 0, buf = 0;  // tiles so far; the query buffer of the next one-tile item
+    bool ahead = false;  // its rows are on the way
+    bool more = get_item(p, j, 0, it);
+    for (int idx = 0; ok && more; ++idx) {
+      const Item now = it;
+      more = get_item(p, j, idx + 1, it);
+      if (now.n == 0) continue;
+      if (now.two) {
+        load_q(0, now.seq0);
+        load_q(1, now.seq0 + TQ);
+        ok = tc::wait_warp(&sm.q_full[0], (qn[0] - 1) & 1, abort) && tc::wait_warp(&sm.q_full[1], (qn[1] - 1) & 1, abort);
+        if (ok) ok = full(g, 0);
+        if (ok && tc::elect()) {
           tc::fence_after();
-          qk(0, 0, 0);
-          qk(1, 1, 0);
-          tc::commit(&sm.kv_empty[0]);
+          qk(0, 0, g);
+          qk(1, 1, g);
+          tc::commit(&sm.kv_empty[2 * (g & 1)]);
         }
-        for (int i = 0; i < n && ok; ++i) {
-          const int cv = 2 * i + 1, ck = 2 * i + 2;
-          ok = full(cv);
-          if (ok && i + 1 < n) ok = full(ck);
+        for (int i = 0; i < now.n && ok; ++i, ++g) {
+          ok = full(g, 1);
+          if (ok && i + 1 < now.n) ok = full(g + 1, 0);
           for (int q = 0; q < 2 && ok; ++q) {
-            ok = tc::wait_warp(&sm.p_full[q], i & 1, abort);
-            if (ok && lane == 0) {
+            ok = p_wait(q);
+            if (ok && tc::elect()) {
               tc::fence_after();
-              pv(q, cv % STAGES, i > 0);
-              if (i + 1 < n) qk(q, q, ck % STAGES);
+              pv(q, g, i > 0);
+              if (i + 1 < now.n) qk(q, q, g + 1);
               else tc::commit(&sm.o_full[q]);
             }
             __syncwarp();
           }
-          if (ok && lane == 0) {
-            tc::commit(&sm.kv_empty[cv % STAGES]);
-            if (i + 1 < n) tc::commit(&sm.kv_empty[ck % STAGES]);
+          if (ok && tc::elect()) {
+            tc::commit(&sm.kv_empty[2 * (g & 1) + 1]);
+            if (i + 1 < now.n) tc::commit(&sm.kv_empty[2 * ((g + 1) & 1)]);
           }
           __syncwarp();
         }
       } else {
         // key tile i belongs to stream i & 1
-        for (int i = 0; i < 2 && i < n && ok; ++i) {
-          ok = full(2 * i);
-          if (ok && lane == 0) {
+        if (!ahead) load_q(buf, now.seq0);
+        ok = tc::wait_warp(&sm.q_full[buf], (qn[buf] - 1) & 1, abort);
+        for (int i = 0; i < 2 && i < now.n && ok; ++i) {
+          ok = full(g + i, 0);
+          if (ok && tc::elect()) {
             tc::fence_after();
-            qk(i, 0, (2 * i) % STAGES);
-            tc::commit(&sm.kv_empty[(2 * i) % STAGES]);
+            qk(i, buf, g + i);
+            tc::commit(&sm.kv_empty[2 * ((g + i) & 1)]);
           }
           __syncwarp();
         }
-        for (int i = 0; i < n && ok; ++i) {
-          const int q = i & 1, cv = 2 * i + 1, ck = 2 * (i + 2);
-          ok = full(cv);
-          if (ok) ok = tc::wait_warp(&sm.p_full[q], (i >> 1) & 1, abort);
-          if (ok && lane == 0) {
+        ahead = more && it.n > 0 && !it.two;
+        if (ahead) load_q(buf ^ 1, it.seq0);  // the item before last is complete
+        for (int i = 0; i < now.n && ok; ++i, ++g) {
+          const int q = i & 1;
+          ok = full(g, 1) && p_wait(q);
+          if (ok && tc::elect()) {
             tc::fence_after();
-            pv(q, cv % STAGES, i > 1);
-            tc::commit(&sm.kv_empty[cv % STAGES]);
-            if (i + 2 >= n) tc::commit(&sm.o_full[q]);
+            pv(q, g, i > 1);
+            tc::commit(&sm.kv_empty[2 * (g & 1) + 1]);
+            if (i + 2 >= now.n) tc::commit(&sm.o_full[q]);
           }
           __syncwarp();
-          if (ok && i + 2 < n) {
-            ok = full(ck);
-            if (ok && lane == 0) {
+          if (ok && i + 2 < now.n) {
+            ok = full(g + 2, 0);
+            if (ok && tc::elect()) {
               tc::fence_after();
-              qk(q, 0, ck % STAGES);
-              tc::commit(&sm.kv_empty[ck % STAGES]);
+              qk(q, buf, g + 2);
+              tc::commit(&sm.kv_empty[2 * (g & 1)]);
             }
             __syncwarp();
           }
         }
+        buf ^= 1;
       }
-      if (lane == 0) tc::commit(&sm.drain);  // no product may be in flight when TMEM is freed
-      __syncwarp();
-      (void)mbar_wait(&sm.drain, 0);
-    } else if (warp == 17 && lane == 0) {
-      // ---- query tiles: TQ sequences x G heads
-      const int nq = two ? 2 : 1;
-      for (int q = 0; q < nq; ++q) {
-        mbar_arrive_expect_tx(&sm.q_full[q], TQ * G * D * 2);
-        for (int u = 0; u < 2; ++u) tc::tma3(sm.q[q] + u * HALF, &p.mq, 64 * u, h * G, seq0 + q * TQ, &sm.q_full[q]);
-      }
-      for (int q = 0; q < nq; ++q) (void)mbar_wait(&sm.q_full[q], 0);  // landed before the CTA's memory goes
+    }
+    for (int b = 0; b < 2; ++b)  // loads still in flight after a timeout land before the CTA's memory goes
+      if (qn[b]) (void)mbar_wait(&sm.q_full[b], (qn[b] - 1) & 1);
+    if (tc::elect()) tc::commit(&sm.drain);  // and no product may be in flight when TMEM is freed
+    __syncwarp();
+    (void)mbar_wait(&sm.drain, 0);
     }
   }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 16) tc::tmem_dealloc(tmem, 512);
+  if (warp == 24) tc::tmem_dealloc(tmem, 512);
   if (threadIdx.x == 0 && sm.abort) set_err(p.err, HX_DEV_ERR_TIMEOUT);
 }
 
@@ -700,7 +749,9 @@ HX_API int hx_prefix_decode(void* stream, const hx_pool_layer* pool, const hx_la
   p.part_o = reinterpret_cast<float*>(scratch);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)(2 * n_splits + 2) * rows * px::D);
   p.err = dev_err;
-  const int64_t grid = (int64_t)H * p.RB * n_splits + (int64_t)B * H;
+  // a CTA for each split of each row block and head; without a prefix, about one an SM
+  p.J = n_splits > 0 ? p.RB * n_splits : (B < 148 / H ? B : (148 / H > 0 ? 148 / H : 1));
+  const int64_t grid = (int64_t)H * p.J;
   if (grid > 0x7fffffffll || rows > 0x7fffffffll) return HX_ERR_UNSUPPORTED;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   constexpr int smem = (int)sizeof(px::Smem) + 1024;

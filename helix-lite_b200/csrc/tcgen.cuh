@@ -36,6 +36,14 @@ HX_DEVINL bool wait_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abor
   return __all_sync(0xffffffffu, wait(bar, parity, abort));
 }
 
+// One lane of the (converged) warp, the same at every call: the thread that
+// issues the products.
+HX_DEVINL bool elect() {
+  uint32_t y;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(y));
+  return y != 0u;
+}
+
 HX_DEVINL void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
