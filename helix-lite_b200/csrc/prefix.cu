@@ -758,10 +758,8 @@ HX_API int hx_prefix_decode(void* stream, const hx_pool_layer* pool, const hx_la
   static_assert(smem <= 232448, "a CTA has 227 KB of shared memory");
   auto kern = pool->bits_k == 4 ? (pool->bits_v == 4 ? px::prefix_kernel<4, 4> : px::prefix_kernel<4, 2>)
                                 : (pool->bits_v == 4 ? px::prefix_kernel<2, 4> : px::prefix_kernel<2, 2>);
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return HX_ERR_LAUNCH;
-  }
+  static unsigned long long done[4] = {0, 0, 0, 0};
+  if (!allow_smem(kern, smem, done[(pool->bits_k == 4) * 2 + (pool->bits_v == 4)])) return HX_ERR_LAUNCH;
   kern<<<(unsigned)grid, px::NTHREADS, smem, s>>>(p);
   HX_LAUNCH_CHECK();
   px::MergeParams mp{p.part_o, p.part_ml, seq_lens, B, H * group, prefix_pages * px::S, n_splits, bt_stride, out,

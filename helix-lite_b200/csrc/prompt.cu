@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
   } else {
     tc::regs_dec<72>();
     if (warp == 8) {
-      // ---- matrix products (one thread issues)
+      // ---- matrix products, issued by one elected lane (elect.sync tells the compiler that a single lane runs:
+      // 1124 against 1037 TFLOP/s at 20K tokens with a test of the lane number)
       constexpr uint32_t ids = tc::idesc_f16(BF16, ROWS, KT, 0), idv = tc::idesc_f16(BF16, ROWS, D, 1);
       auto qk = [&](int q, int stage) {
         const uint32_t qa = smem_u32(sm.q[q]), ka = smem_u32(sm.kv[stage]);
@@ -283,10 +284,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
       bool ok = tc::wait_warp(&sm.kv_full[0], 0, abort);
       for (int q = 0; q < nq && ok; ++q) {
         ok = tc::wait_warp(&sm.q_full[q], 0, abort);
-        if (ok && lane == 0) qk(q, 0);
+        if (ok && tc::elect()) qk(q, 0);
         __syncwarp();
       }
-      if (ok && lane == 0) tc::commit(&sm.kv_empty[0]);
+      if (ok && tc::elect()) tc::commit(&sm.kv_empty[0]);
       for (int i = 0; i < n && ok; ++i) {
         const int cv = 2 * i + 1, ck = 2 * i + 2, sv = cv % STAGES, sk = ck % STAGES;
         ok = tc::wait_warp(&sm.kv_full[sv], (cv / STAGES) & 1, abort);
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
         for (int q = 0; q < nq && ok; ++q) {
           ok = tc::wait_warp(&sm.p_full[q], i & 1, abort);
           if (ok && q == 0 && i >= i_mask) ok = tc::wait_warp(&sm.v_clean, (i - i_mask) & 1, abort);
-          if (ok && lane == 0) {
+          if (ok && tc::elect()) {
             tc::fence_after();
 #pragma unroll
             for (int k = 0; k < KT / 16; ++k)
@@ -307,13 +308,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
           }
           __syncwarp();
         }
-        if (ok && lane == 0) {
+        if (ok && tc::elect()) {
           tc::commit(&sm.kv_empty[sv]);
           if (i + 1 < n) tc::commit(&sm.kv_empty[sk]);
         }
         __syncwarp();
       }
-      if (lane == 0) tc::commit(&sm.drain);  // no product may be in flight when TMEM is freed
+      if (tc::elect()) tc::commit(&sm.drain);  // no product may be in flight when TMEM is freed
       __syncwarp();
       (void)mbar_wait(&sm.drain, 0);
     } else if (warp == 9) {
@@ -392,10 +393,8 @@ template <int D, bool BF16>
 int launch(const Params& p, int64_t grid, cudaStream_t s) {
   constexpr int smem = (int)sizeof(Smem<D>) + 1024;
   static_assert(smem <= 232448, "a CTA has 227 KB of shared memory");
-  if (cudaFuncSetAttribute(prompt_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return HX_ERR_LAUNCH;
-  }
+  static unsigned long long done = 0;
+  if (!allow_smem(prompt_kernel<D, BF16>, smem, done)) return HX_ERR_LAUNCH;
   prompt_kernel<D, BF16><<<(unsigned)grid, NTHREADS, smem, s>>>(p);
   HX_LAUNCH_CHECK();
   return HX_OK;

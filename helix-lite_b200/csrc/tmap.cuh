@@ -36,4 +36,19 @@ inline bool make_tmap3(CUtensorMap* m, bool bf16, const void* base, int D, int h
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Dynamic shared memory above 48 KB, asked for once per kernel and device.
+template <typename K>
+inline bool allow_smem(K kern, int bytes, unsigned long long& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+  return true;
+}
+
 }  // namespace hx

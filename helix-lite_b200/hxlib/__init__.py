@@ -163,6 +163,30 @@ def stream(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+class _Stay:
+    """The device is current already."""
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_STAY = _Stay()
+
+
+def on(index: int):
+    """Context with CUDA device ``index`` current; nothing to do where it is
+    (torch.cuda.device costs a few microseconds either way, as much as a
+    small kernel)."""
+    return _STAY if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def raw_stream(index: int) -> int:
+    """Handle of device ``index``'s current stream."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
@@ -173,6 +197,12 @@ def require_cuda(*tensors):
 
 _err_words: dict = {}
 _scratch: dict = {}
+
+
+def err_ptr(index: int) -> int:
+    """Address of device ``index``'s error word."""
+    w = _err_words.get(index)
+    return (w if w is not None else err_word(torch.device("cuda", index))).data_ptr()
 
 
 def err_word(device) -> torch.Tensor:

@@ -53,6 +53,8 @@ class Selection:
 
 
 def _i32(t, device):
+    if t.dtype == torch.int32 and t.device == device and t.is_contiguous():
+        return t
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
@@ -382,24 +384,25 @@ def shared_prefix_decode(pool: CompactKVPool, layer_idx: int, query: torch.Tenso
     sl = _i32(seq_lens, dev)
     scale = float(softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D))
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=torch.float16, device=dev)
+        out = q.new_empty((B, Hq, D))
     elif out.shape != q.shape or out.dtype != torch.float16 or out.device != q.device or not out.is_contiguous() \
             or out.data_ptr() % 8:
         raise ValueError(f"out must be a contiguous {tuple(q.shape)} float16 tensor on {dev}")
     if lse is None:
-        lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+        lse = q.new_empty((B, Hq), dtype=torch.float32)
     elif lse.shape != (B, Hq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous {(B, Hq)} float32 tensor on {dev}")
     L = hxlib.lib()
+    i = q.device.index
     ns = int(n_splits) if n_splits is not None else L.hx_prefix_splits(B, H, Hq // H, prefix_len // S)
     # from torch's allocator, so calls on different streams or in different captured graphs never share it
-    scr = torch.empty((max(16, L.hx_prefix_scratch_bytes(B, H, Hq // H, ns)),), dtype=torch.uint8, device=dev)
+    scr = q.new_empty(max(16, L.hx_prefix_scratch_bytes(B, H, Hq // H, ns)), dtype=torch.uint8)
     st_scales, _keep = pool.scales.device_layer(layer_idx, dev)
-    with torch.cuda.device(dev):
-        call("hx_prefix_decode", stream(dev), ctypes_ref(pool.layers[layer_idx].struct), ctypes_ref(st_scales), ptr(q), B,
-             Hq // H, scale, ptr(bt), bt.shape[1], ptr(sl), prefix_len // S,
-             hxlib.VPOS_PHYSICAL if v_pos == "physical" else 0, ns, ptr(scr), ptr(out), ptr(lse),
-             ptr(hxlib.err_word(dev)))
+    with hxlib.on(i):
+        call("hx_prefix_decode", hxlib.raw_stream(i), ctypes_ref(pool.layers[layer_idx].struct), ctypes_ref(st_scales),
+             q.data_ptr(), B, Hq // H, scale, bt.data_ptr(), bt.shape[1], sl.data_ptr(), prefix_len // S,
+             hxlib.VPOS_PHYSICAL if v_pos == "physical" else 0, ns, scr.data_ptr(), out.data_ptr(), lse.data_ptr(),
+             hxlib.err_ptr(i))
     return out, lse
 
 
@@ -458,21 +461,23 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         raise ValueError("query, key and value must be on one device")
     scale = float(softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D))
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=query.dtype, device=dev)
+        out = query.new_empty((T, Hq, D))
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous {tuple(query.shape)} {query.dtype} tensor on {dev}")
     if lse is None:
-        lse = torch.empty((T, Hq), dtype=torch.float32, device=dev)
+        lse = query.new_empty((T, Hq), dtype=torch.float32)
     elif lse.shape != (T, Hq) or lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous {(T, Hq)} float32 tensor on {dev}")
     qs = _i32(query_start, dev)
     q, qt, qh = _rows(query)
     k, kt, kh = _rows(key)
     v, vt, vh = _rows(value)
-    with torch.cuda.device(dev):
-        call("hx_prompt_attn", stream(dev), _PROMPT_DT[query.dtype], ptr(q), qt, qh, ptr(k), kt, kh, ptr(v), vt, vh,
-             ptr(qs), qs.numel() - 1, T, H, Hq // H, D, scale, ptr(out), ptr(lse), ptr(hxlib.err_word(dev)))
+    i = dev.index
+    with hxlib.on(i):
+        call("hx_prompt_attn", hxlib.raw_stream(i), _PROMPT_DT[query.dtype], q.data_ptr(), qt, qh, k.data_ptr(), kt, kh,
+             v.data_ptr(), vt, vh, qs.data_ptr(), qs.shape[0] - 1, T, H, Hq // H, D, scale, out.data_ptr(),
+             lse.data_ptr(), hxlib.err_ptr(i))
     return out, lse
 
 

@@ -31,7 +31,7 @@ from dataclasses import dataclass
 import torch
 
 import hxlib
-from hxlib import call, ptr, stream
+from hxlib import call
 
 
 @dataclass
@@ -44,33 +44,42 @@ class BatchTables:
 
 
 def _check(block_table, page_size, num_pages, free_pages, free_count, page_refs, **vectors):
+    """Shapes, types and places; returns the number of pool pages."""
+    dev = block_table.device
+    if dev.type != "cuda":
+        hxlib.require_cuda(block_table)
     if block_table.dim() != 2:
         raise ValueError(f"block_table should be (B, max_pages), got {tuple(block_table.shape)}")
-    named = {"block_table": block_table, "free_pages": free_pages, "free_count": free_count, **vectors}
+    B, W = block_table.shape
+    if block_table.dtype != _I32:
+        raise TypeError(f"block_table must be int32, got {block_table.dtype}")
+    vectors["free_pages"], vectors["free_count"] = free_pages, free_count
     if page_refs is not None:
-        named["page_refs"] = page_refs
-    hxlib.require_cuda(*named.values())
-    for name, t in named.items():
-        if t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32, got {t.dtype}")
-        if t.device != block_table.device:
-            raise ValueError(f"{name} is on {t.device}, block_table on {block_table.device}")
-        if name != "block_table" and not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-    B = block_table.shape[0]
-    if block_table.numel() and (block_table.stride(1) != 1 or (B > 1 and block_table.stride(0) < block_table.shape[1])):
-        raise ValueError("block_table rows must be contiguous and must not overlap")
+        vectors["page_refs"] = page_refs
     for name, t in vectors.items():
-        if t.shape != (B,):
-            raise ValueError(f"{name} should be ({B},), got {tuple(t.shape)}")
-    if free_count.numel() != 1 or free_pages.dim() != 1:
-        raise ValueError("free_pages should be one-dimensional and free_count one number")
-    if int(page_size) < 1:
+        if t.dtype != _I32 or t.device != dev or t.dim() != 1 or not t.is_contiguous() \
+                or (name not in _SIZED and t.shape[0] != B):
+            hxlib.require_cuda(t)
+            if t.dtype != _I32:
+                raise TypeError(f"{name} must be int32, got {t.dtype}")
+            if t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, block_table on {dev}")
+            raise ValueError(f"{name} must be contiguous and " +
+                             ("one-dimensional" if name in _SIZED else f"({B},)") + f", got {tuple(t.shape)}")
+    if B and W and (block_table.stride(1) != 1 or (B > 1 and block_table.stride(0) < W)):
+        raise ValueError("block_table rows must be contiguous and must not overlap")
+    if free_count.shape[0] != 1:
+        raise ValueError("free_count should be one number")
+    if page_size < 1:
         raise ValueError("page_size must be at least 1")
-    n = int(num_pages) if num_pages is not None else (page_refs if page_refs is not None else free_pages).numel()
-    if page_refs is not None and (page_refs.dim() != 1 or page_refs.numel() < n):
+    n = int(num_pages) if num_pages is not None else (page_refs if page_refs is not None else free_pages).shape[0]
+    if page_refs is not None and page_refs.shape[0] < n:
         raise ValueError(f"page_refs should hold one count for each of {n} pages")
     return n
+
+
+_I32 = torch.int32
+_SIZED = ("free_pages", "free_count", "page_refs")
 
 
 def _row_stride(block_table):
@@ -106,24 +115,27 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
     T = int(num_tokens)
     if T < 0:
         raise ValueError("num_tokens must not be negative")
-    want = {"query_start": ((B + 1,), torch.int32), "seq_lens": ((B,), torch.int32), "slot_mapping": ((T,), torch.int64),
-            "positions": ((T,), torch.int64), "free_count": ((1,), torch.int32)}
     if out is None:
-        out = BatchTables(*(torch.empty(s, dtype=d, device=dev) for s, d in want.values()))
+        i32, i64 = free_count.new_empty, torch.int64
+        out = BatchTables(i32(B + 1), i32(B), i32(T, dtype=i64), i32(T, dtype=i64), i32(1))
     else:
         ins = {t.data_ptr() for t in (cached_lens, new_tokens, free_count, free_pages, block_table) if t.numel()}
-        for name, (shape, dt) in want.items():
+        for name, n, dt in (("query_start", B + 1, torch.int32), ("seq_lens", B, torch.int32),
+                            ("slot_mapping", T, torch.int64), ("positions", T, torch.int64),
+                            ("free_count", 1, torch.int32)):
             t = getattr(out, name)
             hxlib.require_cuda(t)
-            if t.shape != shape or t.dtype != dt or t.device != dev or not t.is_contiguous():
-                raise ValueError(f"out.{name} must be a contiguous {shape} {dt} tensor on {dev}")
-            if t.numel() and t.data_ptr() in ins:
+            if t.shape != (n,) or t.dtype != dt or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"out.{name} must be a contiguous ({n},) {dt} tensor on {dev}")
+            if n and t.data_ptr() in ins:
                 raise ValueError(f"out.{name} must not be one of the inputs")
-    with torch.cuda.device(dev):
-        call("hx_tables_extend", stream(dev), ptr(block_table), _row_stride(block_table), B, W, int(page_size),
-             ptr(cached_lens), ptr(new_tokens), ptr(free_pages), free_pages.numel(), ptr(free_count), ptr(page_refs),
-             n_pages, ptr(out.query_start), ptr(out.seq_lens), ptr(out.slot_mapping), ptr(out.positions), T,
-             ptr(out.free_count), ptr(hxlib.err_word(dev)))
+    i = dev.index
+    with hxlib.on(i):
+        call("hx_tables_extend", hxlib.raw_stream(i), block_table.data_ptr(), _row_stride(block_table), B, W,
+             int(page_size), cached_lens.data_ptr(), new_tokens.data_ptr(), free_pages.data_ptr(), free_pages.shape[0],
+             free_count.data_ptr(), page_refs.data_ptr() if page_refs is not None else None, n_pages,
+             out.query_start.data_ptr(), out.seq_lens.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(),
+             T, out.free_count.data_ptr(), hxlib.err_ptr(i))
     return out
 
 
@@ -145,10 +157,11 @@ def truncate_tables(block_table: torch.Tensor, seq_lens: torch.Tensor, keep_lens
                      keep_lens=keep_lens)
     B, W = block_table.shape
     dev = block_table.device
-    lens = torch.empty((B,), dtype=torch.int32, device=dev)
-    count = torch.empty((1,), dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        call("hx_tables_truncate", stream(dev), ptr(block_table), _row_stride(block_table), B, W, int(page_size),
-             ptr(seq_lens), ptr(keep_lens), ptr(free_pages), free_pages.numel(), ptr(free_count), ptr(page_refs),
-             n_pages, ptr(lens), ptr(count), ptr(hxlib.err_word(dev)))
+    lens, count = seq_lens.new_empty(B), free_count.new_empty(1)
+    i = dev.index
+    with hxlib.on(i):
+        call("hx_tables_truncate", hxlib.raw_stream(i), block_table.data_ptr(), _row_stride(block_table), B, W,
+             int(page_size), seq_lens.data_ptr(), keep_lens.data_ptr(), free_pages.data_ptr(), free_pages.shape[0],
+             free_count.data_ptr(), page_refs.data_ptr() if page_refs is not None else None, n_pages, lens.data_ptr(),
+             count.data_ptr(), hxlib.err_ptr(i))
     return lens, count
