@@ -37,12 +37,20 @@ constexpr int ROWS = 128;       // query rows per tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;  // P <= 2^8 before the maximum moves
 
+// A work item: two tiles of query rows of one (sequence, KV head).
+struct Item {
+  int h, s0, len, t0;  // KV head; first row and tokens of the sequence; first token of the item (len 0: no more items)
+};
+
 template <int D>
 struct Smem {
   alignas(1024) uint8_t q[2][ROWS * D * 2];
   alignas(1024) uint8_t kv[STAGES][KT * D * 2];
-  uint64_t q_full[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], v_go, v_clean, drain;
-  uint32_t tmem, abort, bad_v;
+  alignas(16) uint32_t answer[2][4];  // next_cta
+  Item item[2];
+  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], v_go, v_clean;
+  uint64_t item_full[2], item_empty[2], next, drain;
+  uint32_t tmem, abort, bad_v[2];
 };
 
 struct Params {
@@ -90,37 +98,48 @@ HX_DEVINL uint32_t nonfinite2(uint32_t x) {
   constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
   return ((x & e) == e ? 0xFFFFu : 0u) | (((x >> 16) & e) == e ? 0xFFFF0000u : 0u);
 }
+// a * 0 + c on both halves
+template <bool BF16>
+HX_DEVINL uint32_t times_zero(uint32_t a, uint32_t c) {
+  uint32_t r;
+  if (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0u), "r"(c));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0u), "r"(c));
+  return r;
+}
 template <bool BF16>
 HX_DEVINL float to_float(uint16_t x) {
   return BF16 ? __uint_as_float((uint32_t)x << 16) : h2f(x);
 }
+
+// What the roles derive from an item.
+struct Work {
+  int h, s0, len, t0, nq, n, i_mask;  // query tiles with tokens; key tiles; the first of them with masked places
+  HX_DEVINL bool read(const volatile Item& it, int TQ) {
+    h = it.h, s0 = it.s0, len = it.len, t0 = it.t0;
+    nq = t0 + TQ < len ? 2 : 1;
+    n = (min(t0 + 2 * TQ, len) + KT - 1) / KT;
+    i_mask = min((t0 + 1) / KT, n - 1);
+    return len > 0;
+  }
+};
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t raw[];
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x % p.H, slot = (int)(gridDim.x / p.H) - 1 - (int)(blockIdx.x / p.H);
   const int TQ = p.TQ, G = p.G, per = 2 * TQ;
-  const int b = find_seq(p.start, p.B, per, slot);
-  const int s0 = p.start[b], len = p.start[b + 1] - s0;
-  if (s0 < 0 || len < 0 || s0 + len > p.T) {
-    if (threadIdx.x == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
-    return;
-  }
-  const int t0 = (slot - s0 / per - b) * per;  // first token of the CTA, in the sequence
-  if (t0 < 0 || t0 >= len) return;
-  const int nq = t0 + TQ < len ? 2 : 1;        // query tiles with tokens
-  const int n = (min(t0 + per, len) + KT - 1) / KT;
-  const int i_mask = min((t0 + 1) / KT, n - 1);  // first key tile with masked places
 
   if (warp == 8) {
     if (lane == 0) {
       for (int q = 0; q < 2; ++q) {
         mbar_init(&sm.q_full[q], 1);
+        mbar_init(&sm.q_empty[q], 1);
         mbar_init(&sm.s_full[q], 1);
         mbar_init(&sm.p_full[q], 4);
         mbar_init(&sm.o_full[q], 1);
+        mbar_init(&sm.item_full[q], 1);
+        mbar_init(&sm.item_empty[q], 11);  // 8 softmax warps, the MMA warp, 2 V-check warps
       }
       for (int s = 0; s < STAGES; ++s) {
         mbar_init(&sm.kv_full[s], 1);
@@ -128,9 +147,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
       }
       mbar_init(&sm.v_go, 1);
       mbar_init(&sm.v_clean, 2);
+      mbar_init(&sm.next, 1);
       mbar_init(&sm.drain, 1);
       sm.abort = 0u;
-      sm.bad_v = 0u;
       fence_mbar_init();
     }
     __syncwarp();
@@ -148,123 +167,132 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
   volatile uint32_t* abort = &sm.abort;
   constexpr int HALF = KT * 128;  // bytes of 128 rows of 64 elements
   constexpr int NH = D / 64;
+  Work w;
 
   if (warp < 8) {
     // ---- softmax: warpgroup q holds tile q's rows, one a thread
     tc::regs_inc<216>();
     const int q = warp >> 2, r = threadIdx.x & 127;
-    if (q < nq) {
-      const int ti = t0 + q * TQ + r / G;          // token of the row, in the sequence
-      const bool live = r < TQ * G && ti < len;
-      const int tile0 = t0 + q * TQ;               // lowest position of the tile
-      const uint32_t sb = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * q;
-      const uint32_t ob = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 + 128 * q;
-      float m = -INFINITY, l = 0.0f;
-      bool ok = true;
-      for (int i = 0; i < n && ok; ++i) {
-        ok = tc::wait_warp(&sm.s_full[q], i & 1, abort);
-        if (!ok) break;
-        tc::fence_after();
-        uint32_t s[KT];
+    const uint32_t sb = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * q;
+    const uint32_t ob = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 + 128 * q;
+    int used = 0, done = 0;  // S tiles and O results of this warpgroup so far
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      ok = tc::wait_warp(&sm.item_full[it & 1], (it >> 1) & 1, abort);
+      if (!ok || !w.read(sm.item[it & 1], TQ)) break;
+      if (q < w.nq) {
+        const int tile0 = w.t0 + q * TQ;        // lowest position of the tile
+        const int ti = tile0 + r / G;           // token of the row, in the sequence
+        const bool live = r < TQ * G && ti < w.len;
+        float m = -INFINITY, l = 0.0f;
+        for (int i = 0; i < w.n; ++i, ++used) {
+          ok = tc::wait_warp(&sm.s_full[q], used & 1, abort);
+          if (!ok) break;
+          tc::fence_after();
+          uint32_t s[KT];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) tc::ld32(s + 32 * u, sb + 32 * u);
-        tc::wait_ld();
-        if (KT * i + KT - 1 > tile0) {  // masked places: keys past the row's position
-          const int lim = ti - KT * i;
-#pragma unroll
-          for (int j = 0; j < KT; ++j) s[j] = j <= lim ? s[j] : 0xff800000u;
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < KT; j += 8)
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            mx[u] = fmaxf(mx[u], fmaxf(__uint_as_float(s[j + 2 * u]), __uint_as_float(s[j + 2 * u + 1])));
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const bool move = (mt - m) * p.c > kSlack;  // also the first finite maximum (m = -inf)
-        if (__any_sync(0xffffffffu, move)) {
-          const float mn = move ? mt : m;
-          const float a = move ? tc::ex2((m - mn) * p.c) : 1.0f;
-          m = mn;
-          l *= a;
-          if (i > 0) {  // O(i - 1) is complete: S(i) was issued after it
-            const uint64_t a2 = tc::f2_pack(a, a);
-#pragma unroll 1
-            for (int u = 0; u < D / 32; ++u) {
-              uint32_t o[32];
-              tc::ld32(o, ob + 32 * u);
-              tc::wait_ld();
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                float x, y;
-                tc::f2_unpack(tc::f2_mul(tc::f2_pack(__uint_as_float(o[j]), __uint_as_float(o[j + 1])), a2), x, y);
-                o[j] = __float_as_uint(x);
-                o[j + 1] = __float_as_uint(y);
-              }
-              tc::st32(ob + 32 * u, o);
-            }
-          }
-        }
-        const float mb = m == -INFINITY ? 0.0f : -m * p.c;
-        const uint64_t c2 = tc::f2_pack(p.c, p.c), mb2 = tc::f2_pack(mb, mb);
-        uint64_t sum[2] = {0ull, 0ull};
-        uint32_t pk[KT / 2];
-#pragma unroll
-        for (int j = 0; j < KT; j += 2) {
-          float x, y;
-          tc::f2_unpack(tc::f2_fma(tc::f2_pack(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), c2, mb2), x, y);
-          x = tc::ex2(x);
-          y = tc::ex2(y);
-          sum[(j >> 1) & 1] = tc::f2_add(sum[(j >> 1) & 1], tc::f2_pack(x, y));
-          pk[j >> 1] = pack2<BF16>(x, y);
-        }
-        tc::st32(sb, pk);
-        tc::st32(sb + 32, pk + 32);
-        {
-          float x, y;
-          tc::f2_unpack(tc::f2_add(sum[0], sum[1]), x, y);
-          l += x + y;
-        }
-        tc::wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) tc::arrive(&sm.p_full[q]);
-      }
-      // ---- O / l
-      if (ok) ok = tc::wait_warp(&sm.o_full[q], 0, abort);
-      tc::fence_after();
-      if (ok) {
-        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-        const int64_t row = ((int64_t)(s0 + ti) * p.H + h) * G + r % G;
-        const bool bad = sm.bad_v != 0u;
-#pragma unroll 1
-        for (int u = 0; u < D / 32; ++u) {
-          uint32_t o[32];
-          tc::ld32(o, ob + 32 * u);
+          for (int u = 0; u < 4; ++u) tc::ld32(s + 32 * u, sb + 32 * u);
           tc::wait_ld();
-          float f[32];
+          if (KT * i + KT - 1 > tile0) {  // masked places: keys past the row's position
+            const int lim = ti - KT * i;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(o[j]) * inv;
-          if (bad && live) {  // non-finite V that the row sees in the masked tiles
-            for (int key = i_mask * KT; key <= ti; ++key) {
-              const uint16_t* vr = p.v + (int64_t)(s0 + key) * p.v_st + h * p.v_sh + 32 * u;
+            for (int j = 0; j < KT; ++j) s[j] = j <= lim ? s[j] : 0xff800000u;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float x = to_float<BF16>(vr[j]);
-                if (!(fabsf(x) < INFINITY)) f[j] += x;
+          for (int j = 0; j < KT; j += 8)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              mx[u] = fmaxf(mx[u], fmaxf(__uint_as_float(s[j + 2 * u]), __uint_as_float(s[j + 2 * u + 1])));
+          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool move = (mt - m) * p.c > kSlack;  // also the first finite maximum (m = -inf)
+          if (__any_sync(0xffffffffu, move)) {
+            const float mn = move ? mt : m;
+            const float a = move ? tc::ex2((m - mn) * p.c) : 1.0f;
+            m = mn;
+            l *= a;
+            if (i > 0) {  // O(i - 1) is complete: S(i) was issued after it
+              const uint64_t a2 = tc::f2_pack(a, a);
+#pragma unroll 1
+              for (int u = 0; u < D / 32; ++u) {
+                uint32_t o[32];
+                tc::ld32(o, ob + 32 * u);
+                tc::wait_ld();
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                  float x, y;
+                  tc::f2_unpack(tc::f2_mul(tc::f2_pack(__uint_as_float(o[j]), __uint_as_float(o[j + 1])), a2), x, y);
+                  o[j] = __float_as_uint(x);
+                  o[j + 1] = __float_as_uint(y);
+                }
+                tc::st32(ob + 32 * u, o);
               }
             }
           }
-          if (live) {
-            uint4* dst = reinterpret_cast<uint4*>(p.out + row * D + 32 * u);
+          const float mb = m == -INFINITY ? 0.0f : -m * p.c;
+          const uint64_t c2 = tc::f2_pack(p.c, p.c), mb2 = tc::f2_pack(mb, mb);
+          uint64_t sum[2] = {0ull, 0ull};
+          uint32_t pk[KT / 2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              dst[j] = make_uint4(pack2<BF16>(f[8 * j], f[8 * j + 1]), pack2<BF16>(f[8 * j + 2], f[8 * j + 3]),
-                                  pack2<BF16>(f[8 * j + 4], f[8 * j + 5]), pack2<BF16>(f[8 * j + 6], f[8 * j + 7]));
+          for (int j = 0; j < KT; j += 2) {
+            float x, y;
+            tc::f2_unpack(tc::f2_fma(tc::f2_pack(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), c2, mb2), x, y);
+            x = tc::ex2(x);
+            y = tc::ex2(y);
+            sum[(j >> 1) & 1] = tc::f2_add(sum[(j >> 1) & 1], tc::f2_pack(x, y));
+            pk[j >> 1] = pack2<BF16>(x, y);
           }
+          tc::st32(sb, pk);
+          tc::st32(sb + 32, pk + 32);
+          {
+            float x, y;
+            tc::f2_unpack(tc::f2_add(sum[0], sum[1]), x, y);
+            l += x + y;
+          }
+          tc::wait_st();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::arrive(&sm.p_full[q]);
         }
-        if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m * p.c + log2f(l)) * kLn2;
+        // ---- O / l
+        if (ok) ok = tc::wait_warp(&sm.o_full[q], done++ & 1, abort);
+        if (ok) {
+          tc::fence_after();
+          const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+          const int64_t row = ((int64_t)(w.s0 + ti) * p.H + w.h) * G + r % G;
+          const bool bad = *(volatile uint32_t*)&sm.bad_v[it & 1] != 0u;
+#pragma unroll 1
+          for (int u = 0; u < D / 32; ++u) {
+            uint32_t o[32];
+            tc::ld32(o, ob + 32 * u);
+            tc::wait_ld();
+            float f[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(o[j]) * inv;
+            if (bad && live) {  // non-finite V that the row sees in the masked tiles
+              for (int key = w.i_mask * KT; key <= ti; ++key) {
+                const uint16_t* vr = p.v + (int64_t)(w.s0 + key) * p.v_st + w.h * p.v_sh + 32 * u;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                  const float x = to_float<BF16>(vr[j]);
+                  if (!(fabsf(x) < INFINITY)) f[j] += x;
+                }
+              }
+            }
+            if (live) {
+              uint4* dst = reinterpret_cast<uint4*>(p.out + row * D + 32 * u);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                dst[j] = make_uint4(pack2<BF16>(f[8 * j], f[8 * j + 1]), pack2<BF16>(f[8 * j + 2], f[8 * j + 3]),
+                                    pack2<BF16>(f[8 * j + 4], f[8 * j + 5]), pack2<BF16>(f[8 * j + 6], f[8 * j + 7]));
+            }
+          }
+          if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m * p.c + log2f(l)) * kLn2;
+          tc::fence_before();
+        }
       }
+      __syncwarp();
+      if (lane == 0) tc::arrive(&sm.item_empty[it & 1]);
     }
   } else {
     tc::regs_dec<72>();
@@ -281,104 +309,187 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
         }
         tc::commit(&sm.s_full[q]);
       };
-      bool ok = tc::wait_warp(&sm.kv_full[0], 0, abort);
-      for (int q = 0; q < nq && ok; ++q) {
-        ok = tc::wait_warp(&sm.q_full[q], 0, abort);
-        if (ok && tc::elect()) qk(q, 0);
-        __syncwarp();
-      }
-      if (ok && tc::elect()) tc::commit(&sm.kv_empty[0]);
-      for (int i = 0; i < n && ok; ++i) {
-        const int cv = 2 * i + 1, ck = 2 * i + 2, sv = cv % STAGES, sk = ck % STAGES;
-        ok = tc::wait_warp(&sm.kv_full[sv], (cv / STAGES) & 1, abort);
-        if (ok && i >= i_mask && lane == 0) tc::arrive(&sm.v_go);
-        if (ok && i + 1 < n) ok = tc::wait_warp(&sm.kv_full[sk], (ck / STAGES) & 1, abort);
-        const uint32_t va = smem_u32(sm.kv[sv]);
-        for (int q = 0; q < nq && ok; ++q) {
-          ok = tc::wait_warp(&sm.p_full[q], i & 1, abort);
-          if (ok && q == 0 && i >= i_mask) ok = tc::wait_warp(&sm.v_clean, (i - i_mask) & 1, abort);
+      auto full = [&](int c) { return tc::wait_warp(&sm.kv_full[c % STAGES], (c / STAGES) & 1, abort); };
+      int c = 0, vc = 0;             // tiles and checked V tiles so far
+      int qc[2] = {0, 0}, pc[2] = {0, 0};  // items and P tiles of a query tile so far
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        ok = tc::wait_warp(&sm.item_full[it & 1], (it >> 1) & 1, abort);
+        if (!ok || !w.read(sm.item[it & 1], TQ)) break;
+        ok = full(c);
+        for (int q = 0; q < w.nq && ok; ++q) {
+          ok = tc::wait_warp(&sm.q_full[q], qc[q]++ & 1, abort);
           if (ok && tc::elect()) {
             tc::fence_after();
-#pragma unroll
-            for (int k = 0; k < KT / 16; ++k)
-              tc::mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * k, tc::desc128(va + 2048 * k, HALF), idv,
-                         i > 0 || k > 0);
-            if (i + 1 < n) qk(q, sk);
-            else tc::commit(&sm.o_full[q]);
+            qk(q, c % STAGES);
+            if (w.n == 1) tc::commit(&sm.q_empty[q]);
           }
           __syncwarp();
         }
-        if (ok && tc::elect()) {
-          tc::commit(&sm.kv_empty[sv]);
-          if (i + 1 < n) tc::commit(&sm.kv_empty[sk]);
-        }
+        if (ok && tc::elect()) tc::commit(&sm.kv_empty[c % STAGES]);
         __syncwarp();
+        for (int i = 0; i < w.n && ok; ++i) {
+          const int cv = c + 2 * i + 1, ck = cv + 1, sv = cv % STAGES, sk = ck % STAGES;
+          const bool check = i >= w.i_mask;
+          ok = full(cv);
+          if (ok && check && lane == 0) tc::arrive(&sm.v_go);
+          if (ok && i + 1 < w.n) ok = full(ck);
+          const uint32_t va = smem_u32(sm.kv[sv]);
+          for (int q = 0; q < w.nq && ok; ++q) {
+            ok = tc::wait_warp(&sm.p_full[q], pc[q]++ & 1, abort);
+            if (ok && q == 0 && check) ok = tc::wait_warp(&sm.v_clean, vc++ & 1, abort);
+            if (ok && tc::elect()) {
+              tc::fence_after();
+#pragma unroll
+              for (int k = 0; k < KT / 16; ++k)
+                tc::mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * k, tc::desc128(va + 2048 * k, HALF), idv,
+                           i > 0 || k > 0);
+              if (i + 1 < w.n) {
+                qk(q, sk);
+                if (i + 2 == w.n) tc::commit(&sm.q_empty[q]);  // the item's last use of the query tile
+              } else {
+                tc::commit(&sm.o_full[q]);
+              }
+            }
+            __syncwarp();
+          }
+          if (ok && tc::elect()) {
+            tc::commit(&sm.kv_empty[sv]);
+            if (i + 1 < w.n) tc::commit(&sm.kv_empty[sk]);
+          }
+          __syncwarp();
+        }
+        c += 2 * w.n;
+        if (lane == 0) tc::arrive(&sm.item_empty[it & 1]);
       }
       if (tc::elect()) tc::commit(&sm.drain);  // no product may be in flight when TMEM is freed
       __syncwarp();
       (void)mbar_wait(&sm.drain, 0);
     } else if (warp == 9) {
-      // ---- loads: Q tiles, then K0 V0 K1 V1 ...
+      // ---- work items (this CTA's own, then those of CTAs not started yet), and their loads: Q tiles, K0 V0 K1 V1 ...
       bool ok = true;
-      int c = 0;
-      if (lane == 0) {
-        auto load = [&](const CUtensorMap* map, int key) {
-          const int s = c % STAGES;
-          if (c >= STAGES) ok = tc::wait(&sm.kv_empty[s], ((c / STAGES) & 1) ^ 1, abort);
-          if (!ok) return;
-          mbar_arrive_expect_tx(&sm.kv_full[s], KT * D * 2);
+      int c = 0, it = 0, requests = 0, qc[2] = {0, 0};
+      auto load = [&](const CUtensorMap* map, int key) {
+        const int s = c % STAGES;
+        if (c >= STAGES) ok = tc::wait(&sm.kv_empty[s], ((c / STAGES) & 1) ^ 1, abort);
+        if (!ok) return;
+        mbar_arrive_expect_tx(&sm.kv_full[s], KT * D * 2);
 #pragma unroll
-          for (int u = 0; u < NH; ++u) tc::tma3(sm.kv[s] + u * HALF, map, 64 * u, h, s0 + key, &sm.kv_full[s]);
-          ++c;
-        };
-        auto load_q = [&](int q) {
-          mbar_arrive_expect_tx(&sm.q_full[q], TQ * G * D * 2);
+        for (int u = 0; u < NH; ++u) tc::tma3(sm.kv[s] + u * HALF, map, 64 * u, w.h, w.s0 + key, &sm.kv_full[s]);
+        ++c;
+      };
+      auto load_q = [&](int q) {
+        if (qc[q] > 0) ok = tc::wait(&sm.q_empty[q], (qc[q] & 1) ^ 1, abort);
+        if (!ok) return;
+        mbar_arrive_expect_tx(&sm.q_full[q], TQ * G * D * 2);
 #pragma unroll
-          for (int u = 0; u < NH; ++u)
-            tc::tma3(sm.q[q] + u * HALF, &p.mq, 64 * u, h * G, s0 + t0 + q * TQ, &sm.q_full[q]);
-        };
-        load_q(0);
-        load(&p.mk, 0);
-        if (nq > 1) load_q(1);
-        load(&p.mv, 0);
-        for (int i = 1; i < n && ok; ++i) {
-          load(&p.mk, KT * i);
-          if (ok) load(&p.mv, KT * i);
+        for (int u = 0; u < NH; ++u)
+          tc::tma3(sm.q[q] + u * HALF, &p.mq, 64 * u, w.h * G, w.s0 + w.t0 + q * TQ, &sm.q_full[q]);
+        ++qc[q];
+      };
+      int cta = blockIdx.x;
+      for (int asked = 0; ok; ++asked) {
+        if (cta >= 0 && lane == 0) {
+          fence_proxy_async();  // the answer's place was read before
+          tc::next_cta_request(sm.answer[asked & 1], &sm.next);
+          ++requests;
         }
-        if (*abort) {  // given up: let the copies in flight land before the CTA's memory goes
-          for (int q = 0; q < nq; ++q) (void)mbar_wait(&sm.q_full[q], 0);
-          for (int s = max(0, c - STAGES); s < c; ++s) (void)mbar_wait(&sm.kv_full[s % STAGES], (s / STAGES) & 1);
+        Item x = {0, 0, 0, 0};
+        if (cta >= 0) {
+          const int slot = (int)(gridDim.x / p.H) - 1 - cta / p.H;
+          const int b = find_seq(p.start, p.B, per, slot);
+          x.h = cta % p.H;
+          x.s0 = p.start[b];
+          x.len = p.start[b + 1] - x.s0;
+          x.t0 = (slot - x.s0 / per - b) * per;
+          if (x.s0 < 0 || x.len < 0 || x.len > p.T - x.s0) {
+            if (lane == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
+            x.len = 0;
+          }
+          if (x.t0 < 0 || x.t0 >= x.len) x.len = 0;
         }
+        if (x.len > 0 || cta < 0) {  // an item, or the word that there are no more
+          if (it >= 2) ok = tc::wait_warp(&sm.item_empty[it & 1], ((it >> 1) & 1) ^ 1, abort);
+          if (ok && lane == 0) {
+            sm.item[it & 1] = x;
+            sm.bad_v[it & 1] = 0u;
+            tc::arrive(&sm.item_full[it & 1]);
+          }
+          __syncwarp();
+          ++it;
+        }
+        if (cta < 0) break;
+        if (ok && x.len > 0) {
+          w.read(x, TQ);
+          if (lane == 0) {
+            load_q(0);
+            if (ok) load(&p.mk, 0);
+            if (ok && w.nq > 1) load_q(1);
+            if (ok) load(&p.mv, 0);
+            for (int i = 1; i < w.n && ok; ++i) {
+              load(&p.mk, KT * i);
+              if (ok) load(&p.mv, KT * i);
+            }
+          }
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        }
+        if (!tc::wait_warp(&sm.next, asked & 1, abort)) ok = false;
+        cta = ok ? tc::next_cta(sm.answer[asked & 1]) : -1;
+      }
+      if (*abort && lane == 0) {  // given up: let what is in flight land before the CTA's memory goes
+        for (int q = 0; q < 2; ++q)
+          if (qc[q]) (void)mbar_wait(&sm.q_full[q], (qc[q] - 1) & 1);
+        for (int s = max(0, c - STAGES); s < c; ++s) (void)mbar_wait(&sm.kv_full[s % STAGES], (s / STAGES) & 1);
+        if (requests) (void)mbar_wait(&sm.next, (requests - 1) & 1);
       }
       __syncwarp();
     } else {
       // ---- V tiles with masked places: rows past the sequence and non-finite values to 0
-      for (int i = i_mask; i < n; ++i) {
-        const int cv = 2 * i + 1, s = cv % STAGES;
-        // the MMA warp says when the stage holds this tile: these warps see
-        // only some of a stage's phases, so its parity alone could be an older one's
-        if (!tc::wait_warp(&sm.v_go, (i - i_mask) & 1, abort)) break;
-        if (!tc::wait_warp(&sm.kv_full[s], (cv / STAGES) & 1, abort)) break;
-        uint32_t found = 0u;
-        for (int u = (warp - 10) * 32 + lane; u < KT * D / 8; u += 64) {
-          const int key = KT * i + ((u >> 3) & (KT - 1));
-          uint4* at = reinterpret_cast<uint4*>(sm.kv[s]) + u;
-          uint4 x = *at;
-          if (key >= len) {
-            *at = make_uint4(0u, 0u, 0u, 0u);
-          } else {
-            const uint4 e = make_uint4(nonfinite2<BF16>(x.x), nonfinite2<BF16>(x.y), nonfinite2<BF16>(x.z),
-                                       nonfinite2<BF16>(x.w));
-            if (e.x | e.y | e.z | e.w) {
-              found = 1u;
-              *at = make_uint4(x.x & ~e.x, x.y & ~e.y, x.z & ~e.z, x.w & ~e.w);
+      int c = 0, vc = 0;
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        ok = tc::wait_warp(&sm.item_full[it & 1], (it >> 1) & 1, abort);
+        if (!ok || !w.read(sm.item[it & 1], TQ)) break;
+        for (int i = w.i_mask; i < w.n; ++i) {
+          const int cv = c + 2 * i + 1, s = cv % STAGES;
+          // the MMA warp says when the stage holds this tile: these warps see
+          // only some of a stage's phases, so its parity alone could be an older one's
+          ok = tc::wait_warp(&sm.v_go, vc++ & 1, abort) && tc::wait_warp(&sm.kv_full[s], (cv / STAGES) & 1, abort);
+          if (!ok) break;
+          // chunk u: 16 bytes of row (u >> 3) & 127. x * 0 is NaN exactly for a value that is not finite, so a packed
+          // multiply-add per pair looks at a chunk in four instructions (a test of each exponent took 4 us a tile)
+          const int rows = min(KT, w.len - KT * i), first = (warp - 10) * 32 + lane;
+          uint4* tile = reinterpret_cast<uint4*>(sm.kv[s]);
+          uint32_t acc = 0u;
+#pragma unroll 8
+          for (int u = first; u < KT * D / 8; u += 64) {
+            if (((u >> 3) & (KT - 1)) < rows) {
+              const uint4 x = tile[u];
+              acc = times_zero<BF16>(x.x, times_zero<BF16>(x.y, times_zero<BF16>(x.z, times_zero<BF16>(x.w, acc))));
+            } else {
+              tile[u] = make_uint4(0u, 0u, 0u, 0u);
             }
           }
+          uint32_t found = 0u;
+          if (nonfinite2<BF16>(acc)) {
+            for (int u = first; u < KT * D / 8; u += 64) {
+              const uint4 x = tile[u];
+              const uint4 e = make_uint4(nonfinite2<BF16>(x.x), nonfinite2<BF16>(x.y), nonfinite2<BF16>(x.z),
+                                         nonfinite2<BF16>(x.w));
+              if (e.x | e.y | e.z | e.w) {
+                found = 1u;
+                tile[u] = make_uint4(x.x & ~e.x, x.y & ~e.y, x.z & ~e.z, x.w & ~e.w);
+              }
+            }
+          }
+          if (found) sm.bad_v[it & 1] = 1u;
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) tc::arrive(&sm.v_clean);
         }
-        if (found) sm.bad_v = 1u;
-        fence_proxy_async();
+        c += 2 * w.n;
         __syncwarp();
-        if (lane == 0) tc::arrive(&sm.v_clean);
+        if (lane == 0) tc::arrive(&sm.item_empty[it & 1]);
       }
     }
   }

@@ -138,6 +138,34 @@ HX_DEVINL void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
+// ---- taking over CTAs that have not started yet ------------------------------------
+// A running CTA asks the hardware for the next CTA of its own grid that has not
+// been launched (cluster launch control): it cancels that launch and does the
+// work itself, so a grid of one CTA per work item is dealt out dynamically to
+// CTAs that keep their shared memory, TMEM and prefetched tiles. The 16-byte
+// answer lands in shared memory and completes 16 bytes on `bar`.
+HX_DEVINL void next_cta_request(void* answer, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// blockIdx.x taken over, or -1 when the grid has no CTA left
+HX_DEVINL int next_cta(const void* answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n .reg .b64 lo, hi;\n .reg .b128 h;\n .reg .pred p;\n"
+      " ld.shared.v2.b64 {lo, hi}, [%2];\n mov.b128 h, {lo, hi};\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      " selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok ? (int)x : -1;
+}
+
 // ---- register budget of a warpgroup ------------------------------------------------
 template <int N>
 HX_DEVINL void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }

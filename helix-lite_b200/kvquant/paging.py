@@ -45,11 +45,11 @@ class BatchTables:
 
 def _check(block_table, page_size, num_pages, free_pages, free_count, page_refs, **vectors):
     """Shapes, types and places; returns the number of pool pages."""
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table should be (B, max_pages), got {tuple(block_table.shape)}")
     dev = block_table.device
     if dev.type != "cuda":
         hxlib.require_cuda(block_table)
-    if block_table.dim() != 2:
-        raise ValueError(f"block_table should be (B, max_pages), got {tuple(block_table.shape)}")
     B, W = block_table.shape
     if block_table.dtype != _I32:
         raise TypeError(f"block_table must be int32, got {block_table.dtype}")
