@@ -21,7 +21,7 @@
 //
 // Masked places: a masked score is replaced by -inf, never added to, so K there
 // may hold anything. V there meets P = 0 in the product, and 0 * inf is NaN: in
-// the key tiles that hold masked places two warps replace rows past the
+// the key tiles that hold masked places a warp replaces rows past the
 // sequence's end and non-finite values by 0 before the product, and rows
 // allowed to see a non-finite value get it added at the end (P > 0 there).
 #include "tcgen.cuh"
@@ -30,7 +30,7 @@
 namespace hx {
 namespace pr {
 
-constexpr int NTHREADS = 384;   // 2 softmax warpgroups; MMA, load and 2 V-check warps
+constexpr int NTHREADS = 384;   // 2 softmax warpgroups; 2 product warps, the load warp, the V-check warp
 constexpr int STAGES = 5;       // K and V tiles in flight
 constexpr int KT = 128;         // keys per tile
 constexpr int ROWS = 128;       // query rows per tile
@@ -48,7 +48,7 @@ struct Smem {
   alignas(1024) uint8_t kv[STAGES][KT * D * 2];
   alignas(16) uint32_t answer[2][4];  // next_cta
   Item item[2];
-  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], v_go, v_clean;
+  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], turn[2], v_go, v_clean[3];
   uint64_t item_full[2], item_empty[2], next, drain;
   uint32_t tmem, abort, bad_v[2];
 };
@@ -111,6 +111,15 @@ HX_DEVINL float to_float(uint16_t x) {
   return BF16 ? __uint_as_float((uint32_t)x << 16) : h2f(x);
 }
 
+// Stage and parity of every second tile of the ring (K tiles, or V tiles).
+struct Ring {
+  int stage, phase;
+  HX_DEVINL void next() {
+    stage += 2;
+    if (stage >= STAGES) stage -= STAGES, phase ^= 1;
+  }
+};
+
 // What the roles derive from an item.
 struct Work {
   int h, s0, len, t0, nq, n, i_mask;  // query tiles with tokens; key tiles; the first of them with masked places
@@ -138,17 +147,18 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
         mbar_init(&sm.s_full[q], 1);
         mbar_init(&sm.p_full[q], 4);
         mbar_init(&sm.o_full[q], 1);
+        mbar_init(&sm.turn[q], 1);
         mbar_init(&sm.item_full[q], 1);
-        mbar_init(&sm.item_empty[q], 11);  // 8 softmax warps, the MMA warp, 2 V-check warps
+        mbar_init(&sm.item_empty[q], 11);  // 8 softmax warps, 2 product warps, the V-check warp
       }
       for (int s = 0; s < STAGES; ++s) {
         mbar_init(&sm.kv_full[s], 1);
-        mbar_init(&sm.kv_empty[s], 1);
+        mbar_init(&sm.kv_empty[s], 2);  // both query tiles' products
       }
       mbar_init(&sm.v_go, 1);
-      mbar_init(&sm.v_clean, 2);
+      for (int i = 0; i < 3; ++i) mbar_init(&sm.v_clean[i], 1);
       mbar_init(&sm.next, 1);
-      mbar_init(&sm.drain, 1);
+      mbar_init(&sm.drain, 2);
       sm.abort = 0u;
       fence_mbar_init();
     }
@@ -296,70 +306,83 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
     }
   } else {
     tc::regs_dec<72>();
-    if (warp == 8) {
-      // ---- matrix products, issued by one elected lane (elect.sync tells the compiler that a single lane runs:
-      // 1124 against 1037 TFLOP/s at 20K tokens with a test of the lane number)
+    if (warp == 8 || warp == 10) {
+      // ---- matrix products: a warp for each query tile, since issuing blocks (68 cycles a product at 64 of work) and
+      // a wait that is over already still costs 200 to 300: with one warp for both tiles the tensor core stood still
+      // for a third of the time. elect.sync tells the compiler that a single lane runs (a test of the lane number
+      // cost 8%).
+      const int q = warp == 8 ? 0 : 1;
       constexpr uint32_t ids = tc::idesc_f16(BF16, ROWS, KT, 0), idv = tc::idesc_f16(BF16, ROWS, D, 1);
-      auto qk = [&](int q, int stage) {
-        const uint32_t qa = smem_u32(sm.q[q]), ka = smem_u32(sm.kv[stage]);
+      const uint32_t ts = tmem + 128 * q, to = tmem + 256 + 128 * q;
+      Ring rk = {0, 0}, rv = {1, 0};  // stages of the next K and V tile
+      int vc = 0, qc = 0, pc = 0, turns = 0;  // checked V tiles, items, P tiles and turns so far
+      if (q == 1 && lane == 0) tc::arrive(&sm.turn[0]);
+      auto qk = [&](int stage) {
+        const uint32_t qa = smem_u32(sm.q[q]), ka = smem_u32(sm.kv[0]) + stage * (KT * D * 2);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t off = (k / 4) * HALF + (k % 4) * 32;
-          tc::mma_ss(tmem + 128 * q, tc::desc128(qa + off, 0), tc::desc128(ka + off, 0), ids, k > 0);
+          tc::mma_ss(ts, tc::desc128(qa + off, 0), tc::desc128(ka + off, 0), ids, k > 0);
         }
         tc::commit(&sm.s_full[q]);
+        tc::commit(&sm.kv_empty[stage]);
       };
-      auto full = [&](int c) { return tc::wait_warp(&sm.kv_full[c % STAGES], (c / STAGES) & 1, abort); };
-      int c = 0, vc = 0;             // tiles and checked V tiles so far
-      int qc[2] = {0, 0}, pc[2] = {0, 0};  // items and P tiles of a query tile so far
+      // checked tile m completes barrier m % 3. One tile's warp may be two tiles ahead of the other's, not three (the
+      // ring has STAGES < 6 stages), so neither warp meets a barrier one phase too early or too late
+      static_assert(STAGES < 6, "three barriers for checked tiles");
+      auto v_clean = [&](int m) { return tc::wait_warp(&sm.v_clean[m % 3], (m / 3) & 1, abort); };
+      auto full = [&](const Ring& r) { return tc::wait_warp(&sm.kv_full[r.stage], r.phase, abort); };
       bool ok = true;
       for (int it = 0; ok; ++it) {
         ok = tc::wait_warp(&sm.item_full[it & 1], (it >> 1) & 1, abort);
         if (!ok || !w.read(sm.item[it & 1], TQ)) break;
-        ok = full(c);
-        for (int q = 0; q < w.nq && ok; ++q) {
-          ok = tc::wait_warp(&sm.q_full[q], qc[q]++ & 1, abort);
+        if (q >= w.nq) {  // no rows: only give the tiles back
+          for (int i = 0; i < 2 * w.n && ok; ++i) {
+            Ring& r = i & 1 ? rv : rk;
+            ok = full(r);
+            if (ok && lane == 0) tc::arrive(&sm.kv_empty[r.stage]);
+            r.next();
+          }
+        } else {
+          ok = full(rk) && tc::wait_warp(&sm.q_full[q], qc++ & 1, abort);
           if (ok && tc::elect()) {
             tc::fence_after();
-            qk(q, c % STAGES);
+            qk(rk.stage);
             if (w.n == 1) tc::commit(&sm.q_empty[q]);
           }
           __syncwarp();
-        }
-        if (ok && tc::elect()) tc::commit(&sm.kv_empty[c % STAGES]);
-        __syncwarp();
-        for (int i = 0; i < w.n && ok; ++i) {
-          const int cv = c + 2 * i + 1, ck = cv + 1, sv = cv % STAGES, sk = ck % STAGES;
-          const bool check = i >= w.i_mask;
-          ok = full(cv);
-          if (ok && check && lane == 0) tc::arrive(&sm.v_go);
-          if (ok && i + 1 < w.n) ok = full(ck);
-          const uint32_t va = smem_u32(sm.kv[sv]);
-          for (int q = 0; q < w.nq && ok; ++q) {
-            ok = tc::wait_warp(&sm.p_full[q], pc[q]++ & 1, abort);
-            if (ok && q == 0 && check) ok = tc::wait_warp(&sm.v_clean, vc++ & 1, abort);
+          rk.next();
+          for (int i = 0; i < w.n && ok; ++i) {
+            const bool more = i + 1 < w.n, check = i >= w.i_mask;
+            ok = full(rv);
+            if (ok && check && q == 0 && lane == 0) tc::arrive(&sm.v_go);
+            if (ok && more) ok = full(rk);
+            if (ok && check) ok = v_clean(vc++);
+            if (ok) ok = tc::wait_warp(&sm.p_full[q], pc++ & 1, abort);
+            // the tiles take turns, PV and S of one in a row: left to interleave, both finish together, both
+            // softmaxes run together, and the tensor core waits for them (4280 cycles a key tile)
+            if (ok && w.nq == 2) ok = tc::wait_warp(&sm.turn[q], turns++ & 1, abort);
             if (ok && tc::elect()) {
               tc::fence_after();
+              const uint32_t va = smem_u32(sm.kv[0]) + rv.stage * (KT * D * 2);
 #pragma unroll
               for (int k = 0; k < KT / 16; ++k)
-                tc::mma_ts(tmem + 256 + 128 * q, tmem + 128 * q + 8 * k, tc::desc128(va + 2048 * k, HALF), idv,
-                           i > 0 || k > 0);
-              if (i + 1 < w.n) {
-                qk(q, sk);
+                tc::mma_ts(to, ts + 8 * k, tc::desc128(va + 2048 * k, HALF), idv, i > 0 || k > 0);
+              tc::commit(&sm.kv_empty[rv.stage]);
+              if (more) {
+                qk(rk.stage);
                 if (i + 2 == w.n) tc::commit(&sm.q_empty[q]);  // the item's last use of the query tile
               } else {
                 tc::commit(&sm.o_full[q]);
               }
             }
             __syncwarp();
+            if (ok && w.nq == 2 && lane == 0) tc::arrive(&sm.turn[q ^ 1]);
+            rv.next();
+            if (more) rk.next();
           }
-          if (ok && tc::elect()) {
-            tc::commit(&sm.kv_empty[sv]);
-            if (i + 1 < w.n) tc::commit(&sm.kv_empty[sk]);
-          }
-          __syncwarp();
         }
-        c += 2 * w.n;
+        if (q >= w.nq) vc += w.n - w.i_mask;
         if (lane == 0) tc::arrive(&sm.item_empty[it & 1]);
       }
       if (tc::elect()) tc::commit(&sm.drain);  // no product may be in flight when TMEM is freed
@@ -452,17 +475,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
         if (!ok || !w.read(sm.item[it & 1], TQ)) break;
         for (int i = w.i_mask; i < w.n; ++i) {
           const int cv = c + 2 * i + 1, s = cv % STAGES;
-          // the MMA warp says when the stage holds this tile: these warps see
+          // a product warp says when the stage holds this tile: this warp sees
           // only some of a stage's phases, so its parity alone could be an older one's
-          ok = tc::wait_warp(&sm.v_go, vc++ & 1, abort) && tc::wait_warp(&sm.kv_full[s], (cv / STAGES) & 1, abort);
+          ok = tc::wait_warp(&sm.v_go, vc & 1, abort) && tc::wait_warp(&sm.kv_full[s], (cv / STAGES) & 1, abort);
           if (!ok) break;
           // chunk u: 16 bytes of row (u >> 3) & 127. x * 0 is NaN exactly for a value that is not finite, so a packed
           // multiply-add per pair looks at a chunk in four instructions (a test of each exponent took 4 us a tile)
-          const int rows = min(KT, w.len - KT * i), first = (warp - 10) * 32 + lane;
+          const int rows = min(KT, w.len - KT * i), first = lane;
           uint4* tile = reinterpret_cast<uint4*>(sm.kv[s]);
           uint32_t acc = 0u;
 #pragma unroll 8
-          for (int u = first; u < KT * D / 8; u += 64) {
+          for (int u = first; u < KT * D / 8; u += 32) {
             if (((u >> 3) & (KT - 1)) < rows) {
               const uint4 x = tile[u];
               acc = times_zero<BF16>(x.x, times_zero<BF16>(x.y, times_zero<BF16>(x.z, times_zero<BF16>(x.w, acc))));
@@ -472,7 +495,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
           }
           uint32_t found = 0u;
           if (nonfinite2<BF16>(acc)) {
-            for (int u = first; u < KT * D / 8; u += 64) {
+            for (int u = first; u < KT * D / 8; u += 32) {
               const uint4 x = tile[u];
               const uint4 e = make_uint4(nonfinite2<BF16>(x.x), nonfinite2<BF16>(x.y), nonfinite2<BF16>(x.z),
                                          nonfinite2<BF16>(x.w));
@@ -485,7 +508,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
           if (found) sm.bad_v[it & 1] = 1u;
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) tc::arrive(&sm.v_clean);
+          if (lane == 0) tc::arrive(&sm.v_clean[vc % 3]);
+          ++vc;
         }
         c += 2 * w.n;
         __syncwarp();
