@@ -31,11 +31,13 @@ namespace hx {
 namespace pr {
 
 constexpr int NTHREADS = 384;   // 2 softmax warpgroups; 2 product warps, the load warp, the V-check warp
-constexpr int STAGES = 5;       // K and V tiles in flight
+constexpr int STAGES = 4;       // K and V tiles in flight
 constexpr int KT = 128;         // keys per tile
 constexpr int ROWS = 128;       // query rows per tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;  // P <= 2^8 before the maximum moves
+
+constexpr int kOutRow = 80;     // bytes of a staged output row: 64, and 16 so that eight rows meet all banks
 
 // A work item: two tiles of query rows of one (sequence, KV head).
 struct Item {
@@ -46,7 +48,8 @@ template <int D>
 struct Smem {
   alignas(1024) uint8_t q[2][ROWS * D * 2];
   alignas(1024) uint8_t kv[STAGES][KT * D * 2];
-  alignas(16) uint32_t answer[2][4];  // next_cta
+  alignas(16) uint8_t out[8][32 * kOutRow];  // 32 columns of a softmax warp's output rows
+  alignas(16) uint32_t answer[2][4];         // next_cta
   Item item[2];
   uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], turn[2], v_go, v_clean[3];
   uint64_t item_full[2], item_empty[2], next, drain;
@@ -185,6 +188,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
     const int q = warp >> 2, r = threadIdx.x & 127;
     const uint32_t sb = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * q;
     const uint32_t ob = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 + 128 * q;
+    const int rt = r / G, rg = r - rt * G;  // token of the row in the tile, head of the group
+    const uint32_t stage = smem_u32(sm.out[warp]);
     int used = 0, done = 0;  // S tiles and O results of this warpgroup so far
     bool ok = true;
     for (int it = 0; ok; ++it) {
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
       if (!ok || !w.read(sm.item[it & 1], TQ)) break;
       if (q < w.nq) {
         const int tile0 = w.t0 + q * TQ;        // lowest position of the tile
-        const int ti = tile0 + r / G;           // token of the row, in the sequence
+        const int ti = tile0 + rt;              // token of the row, in the sequence
         const bool live = r < TQ * G && ti < w.len;
         float m = -INFINITY, l = 0.0f;
         for (int i = 0; i < w.n; ++i, ++used) {
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
         if (ok) {
           tc::fence_after();
           const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-          const int64_t row = ((int64_t)(w.s0 + ti) * p.H + w.h) * G + r % G;
+          const int64_t row = ((int64_t)(w.s0 + ti) * p.H + w.h) * G + rg;
           const bool bad = *(volatile uint32_t*)&sm.bad_v[it & 1] != 0u;
 #pragma unroll 1
           for (int u = 0; u < D / 32; ++u) {
@@ -289,13 +294,27 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
                 }
               }
             }
-            if (live) {
-              uint4* dst = reinterpret_cast<uint4*>(p.out + row * D + 32 * u);
+            // through shared memory, so that four lanes write 64 bytes of a row and a store meets 8 rows, not 32
+            // (a row a lane: 5500 cycles for the tile's output, as long as one and a half key tiles)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                dst[j] = make_uint4(pack2<BF16>(f[8 * j], f[8 * j + 1]), pack2<BF16>(f[8 * j + 2], f[8 * j + 3]),
-                                    pack2<BF16>(f[8 * j + 4], f[8 * j + 5]), pack2<BF16>(f[8 * j + 6], f[8 * j + 7]));
+            for (int j = 0; j < 4; ++j)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * kOutRow + 16 * j),
+                           "r"(pack2<BF16>(f[8 * j], f[8 * j + 1])), "r"(pack2<BF16>(f[8 * j + 2], f[8 * j + 3])),
+                           "r"(pack2<BF16>(f[8 * j + 4], f[8 * j + 5])), "r"(pack2<BF16>(f[8 * j + 6], f[8 * j + 7]))
+                           : "memory");
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int from = 8 * j + (lane >> 2);
+              const int64_t to = __shfl_sync(0xffffffffu, live ? row : -1, from);
+              uint4 x;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                           : "r"(stage + from * kOutRow + 16 * (lane & 3))
+                           : "memory");
+              if (to >= 0) *reinterpret_cast<uint4*>(p.out + to * D + 32 * u + 8 * (lane & 3)) = x;
             }
+            __syncwarp();
           }
           if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m * p.c + log2f(l)) * kLn2;
           tc::fence_before();
@@ -327,8 +346,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
         tc::commit(&sm.s_full[q]);
         tc::commit(&sm.kv_empty[stage]);
       };
-      // checked tile m completes barrier m % 3. One tile's warp may be two tiles ahead of the other's, not three (the
-      // ring has STAGES < 6 stages), so neither warp meets a barrier one phase too early or too late
+      // checked tile m completes barrier m % 3. One query tile's warp may be two key tiles ahead of the other's, not
+      // three (the ring has STAGES < 6 stages), so neither warp meets a barrier one phase too early or too late
       static_assert(STAGES < 6, "three barriers for checked tiles");
       auto v_clean = [&](int m) { return tc::wait_warp(&sm.v_clean[m % 3], (m / 3) & 1, abort); };
       auto full = [&](const Ring& r) { return tc::wait_warp(&sm.kv_full[r.stage], r.phase, abort); };
@@ -483,18 +502,22 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
           // multiply-add per pair looks at a chunk in four instructions (a test of each exponent took 4 us a tile)
           const int rows = min(KT, w.len - KT * i), first = lane;
           uint4* tile = reinterpret_cast<uint4*>(sm.kv[s]);
-          uint32_t acc = 0u;
+          uint32_t acc[4] = {0u, 0u, 0u, 0u};
 #pragma unroll 8
-          for (int u = first; u < KT * D / 8; u += 32) {
-            if (((u >> 3) & (KT - 1)) < rows) {
-              const uint4 x = tile[u];
-              acc = times_zero<BF16>(x.x, times_zero<BF16>(x.y, times_zero<BF16>(x.z, times_zero<BF16>(x.w, acc))));
-            } else {
-              tile[u] = make_uint4(0u, 0u, 0u, 0u);
-            }
+          for (int u = first; u < KT * D / 8; u += 32) {  // rows to be zeroed are looked at too: at worst once more below
+            const uint4 x = tile[u];
+            acc[0] = times_zero<BF16>(x.x, acc[0]);
+            acc[1] = times_zero<BF16>(x.y, acc[1]);
+            acc[2] = times_zero<BF16>(x.z, acc[2]);
+            acc[3] = times_zero<BF16>(x.w, acc[3]);
           }
+#pragma unroll
+          for (int hf = 0; hf < NH; ++hf)
+            for (int u = hf * (KT * 8) + rows * 8 + lane; u < (hf + 1) * (KT * 8); u += 32)
+              tile[u] = make_uint4(0u, 0u, 0u, 0u);
+          __syncwarp();
           uint32_t found = 0u;
-          if (nonfinite2<BF16>(acc)) {
+          if (nonfinite2<BF16>(acc[0]) | nonfinite2<BF16>(acc[1]) | nonfinite2<BF16>(acc[2]) | nonfinite2<BF16>(acc[3])) {
             for (int u = first; u < KT * D / 8; u += 32) {
               const uint4 x = tile[u];
               const uint4 e = make_uint4(nonfinite2<BF16>(x.x), nonfinite2<BF16>(x.y), nonfinite2<BF16>(x.z),

@@ -24,7 +24,7 @@ HX_DEVINL bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
         : "r"(addr), "r"(parity)
         : "memory");
     if (done) return true;
-    if (*abort) return false;
+    if ((i & 15u) == 15u && *abort) return false;
   }
   *abort = 1u;
   return false;
@@ -33,6 +33,15 @@ HX_DEVINL bool wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
 // The same for a whole warp: one answer for all lanes, since warp-wide
 // (.sync.aligned) instructions follow.
 HX_DEVINL bool wait_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n"
+      " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, done)) return true;
   return __all_sync(0xffffffffu, wait(bar, parity, abort));
 }
 
