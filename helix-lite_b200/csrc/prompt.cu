@@ -51,7 +51,7 @@ struct Smem {
   alignas(16) uint8_t out[8][32 * kOutRow];  // 32 columns of a softmax warp's output rows
   alignas(16) uint32_t answer[2][4];         // next_cta
   Item item[2];
-  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], turn[2], v_go, v_clean[3];
+  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], p_half[2], o_full[2], turn[2], v_go, v_clean[3];
   uint64_t item_full[2], item_empty[2], next, drain;
   uint32_t tmem, abort, bad_v[2];
 };
@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
         mbar_init(&sm.q_empty[q], 1);
         mbar_init(&sm.s_full[q], 1);
         mbar_init(&sm.p_full[q], 4);
+        mbar_init(&sm.p_half[q], 4);
         mbar_init(&sm.o_full[q], 1);
         mbar_init(&sm.turn[q], 1);
         mbar_init(&sm.item_full[q], 1);
@@ -247,27 +248,28 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
           const float mb = m == -INFINITY ? 0.0f : -m * p.c;
           const uint64_t c2 = tc::f2_pack(p.c, p.c), mb2 = tc::f2_pack(mb, mb);
           uint64_t sum[2] = {0ull, 0ull};
-          uint32_t pk[KT / 2];
 #pragma unroll
-          for (int j = 0; j < KT; j += 2) {
-            float x, y;
-            tc::f2_unpack(tc::f2_fma(tc::f2_pack(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), c2, mb2), x, y);
-            x = tc::ex2(x);
-            y = tc::ex2(y);
-            sum[(j >> 1) & 1] = tc::f2_add(sum[(j >> 1) & 1], tc::f2_pack(x, y));
-            pk[j >> 1] = pack2<BF16>(x, y);
+          for (int hf = 0; hf < 2; ++hf) {  // the product over the first 64 keys starts while the others' exponentials run
+            uint32_t pk[KT / 4];
+#pragma unroll
+            for (int j = 0; j < KT / 2; j += 2) {
+              float x, y;
+              tc::f2_unpack(
+                  tc::f2_fma(tc::f2_pack(__uint_as_float(s[64 * hf + j]), __uint_as_float(s[64 * hf + j + 1])), c2, mb2), x, y);
+              x = tc::ex2(x);
+              y = tc::ex2(y);
+              sum[(j >> 1) & 1] = tc::f2_add(sum[(j >> 1) & 1], tc::f2_pack(x, y));
+              pk[j >> 1] = pack2<BF16>(x, y);
+            }
+            tc::st32(sb + 32 * hf, pk);
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::arrive(hf == 0 ? &sm.p_half[q] : &sm.p_full[q]);
           }
-          tc::st32(sb, pk);
-          tc::st32(sb + 32, pk + 32);
-          {
-            float x, y;
-            tc::f2_unpack(tc::f2_add(sum[0], sum[1]), x, y);
-            l += x + y;
-          }
-          tc::wait_st();
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) tc::arrive(&sm.p_full[q]);
+          float x, y;
+          tc::f2_unpack(tc::f2_add(sum[0], sum[1]), x, y);
+          l += x + y;
         }
         // ---- O / l
         if (ok) ok = tc::wait_warp(&sm.o_full[q], done++ & 1, abort);
@@ -377,7 +379,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
             if (ok && check && q == 0 && lane == 0) tc::arrive(&sm.v_go);
             if (ok && more) ok = full(rk);
             if (ok && check) ok = v_clean(vc++);
-            if (ok) ok = tc::wait_warp(&sm.p_full[q], pc++ & 1, abort);
+            if (ok) ok = tc::wait_warp(&sm.p_half[q], pc & 1, abort);
             // the tiles take turns, PV and S of one in a row: left to interleave, both finish together, both
             // softmaxes run together, and the tensor core waits for them (4280 cycles a key tile)
             if (ok && w.nq == 2) ok = tc::wait_warp(&sm.turn[q], turns++ & 1, abort);
@@ -385,8 +387,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
               tc::fence_after();
               const uint32_t va = smem_u32(sm.kv[0]) + rv.stage * (KT * D * 2);
 #pragma unroll
-              for (int k = 0; k < KT / 16; ++k)
+              for (int k = 0; k < KT / 32; ++k)
                 tc::mma_ts(to, ts + 8 * k, tc::desc128(va + 2048 * k, HALF), idv, i > 0 || k > 0);
+            }
+            if (ok) ok = tc::wait_warp(&sm.p_full[q], pc++ & 1, abort);
+            if (ok && tc::elect()) {
+              tc::fence_after();
+              const uint32_t va = smem_u32(sm.kv[0]) + rv.stage * (KT * D * 2);
+#pragma unroll
+              for (int k = KT / 32; k < KT / 16; ++k)
+                tc::mma_ts(to, ts + 8 * k, tc::desc128(va + 2048 * k, HALF), idv, 1);
               tc::commit(&sm.kv_empty[rv.stage]);
               if (more) {
                 qk(rk.stage);
