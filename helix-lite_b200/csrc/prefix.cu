@@ -68,8 +68,10 @@ HX_DEVINL uint32_t pack_h2(float lo, float hi) {
   return r;
 }
 
-// A CTA's items: its split of the prefix, then the suffixes of sequences j, j +
-// J, ... (j the CTA's place among the J of its head). Every role walks them alike.
+// A CTA's items: its split of the prefix, if it has one, then suffixes. j is the
+// CTA's place among the J of its head; the first RB * n_splits have a split,
+// and sequence b's suffix is CTA (RB * n_splits + b) mod J's, so that CTAs
+// without a split take theirs first. Every role walks the items alike.
 struct Item {
   int seq0, page0, pages, tokens, pidx, n;  // first sequence of the rows; pages [page0, page0 + pages) of table row trow
   int64_t trow;
@@ -77,7 +79,7 @@ struct Item {
 };
 
 HX_DEVINL bool get_item(const Params& p, int j, int idx, Item& it) {
-  const int lead = p.n_splits > 0 ? 1 : 0;
+  const int pre = p.RB * p.n_splits, lead = j < pre ? 1 : 0;
   if (idx < lead) {
     const int rb = j % p.RB, split = j / p.RB;
     it.suffix = false;
@@ -91,7 +93,8 @@ HX_DEVINL bool get_item(const Params& p, int j, int idx, Item& it) {
     it.pidx = 2 * split;
     it.trow = 0;
   } else {
-    const int b = j + (idx - lead) * p.J;
+    const int first = j - pre % p.J;
+    const int b = (first < 0 ? first + p.J : first) + (idx - lead) * p.J;
     if (b >= p.B) return false;
     const int len = p.seq_lens[b];
     it.suffix = true;
@@ -684,8 +687,12 @@ __global__ void __launch_bounds__(32 * MW) merge_kernel(const MergeParams p) {
   }
 }
 
+// Splits of the prefix: CTAs for one wave (one fits an SM), at most one split
+// per key tile. Holding CTAs back for the suffixes (two key tiles a sequence
+// assumed, since their lengths are not known on the host) was slower: 32K
+// tokens and 64 suffixes of up to 512 took 91 us against 84, 128K and 16 of up
+// to 777 85 against 81.
 int default_splits(int H, int RB, int tiles) {
-  // one wave of prefix CTAs (one fits an SM); at most one split per key tile
   int ns = 148 / (H * RB);
   ns = ns < 1 ? 1 : ns;
   return ns > tiles ? tiles : ns;
@@ -749,8 +756,9 @@ HX_API int hx_prefix_decode(void* stream, const hx_pool_layer* pool, const hx_la
   p.part_o = reinterpret_cast<float*>(scratch);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)(2 * n_splits + 2) * rows * px::D);
   p.err = dev_err;
-  // a CTA for each split of each row block and head; without a prefix, about one an SM
-  p.J = n_splits > 0 ? p.RB * n_splits : (B < 148 / H ? B : (148 / H > 0 ? 148 / H : 1));
+  // a CTA for each split of each row block and head, and more for the suffixes while SMs are left
+  const int pre = p.RB * n_splits, wave = 148 / H > 1 ? 148 / H : 1;
+  p.J = pre + B < wave ? pre + B : (pre > wave ? pre : wave);
   const int64_t grid = (int64_t)H * p.J;
   if (grid > 0x7fffffffll || rows > 0x7fffffffll) return HX_ERR_UNSUPPORTED;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
