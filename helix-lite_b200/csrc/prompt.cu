@@ -51,7 +51,7 @@ struct Smem {
   alignas(16) uint8_t out[8][32 * kOutRow];  // 32 columns of a softmax warp's output rows
   alignas(16) uint32_t answer[2][4];         // next_cta
   Item item[2];
-  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], p_half[2], o_full[2], turn[2], v_go, v_clean[3];
+  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], p_half[2], o_full[2], turn[2], v_clean[3];
   uint64_t item_full[2], item_empty[2], next, drain;
   uint32_t tmem, abort, bad_v[2];
 };
@@ -157,9 +157,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
       }
       for (int s = 0; s < STAGES; ++s) {
         mbar_init(&sm.kv_full[s], 1);
-        mbar_init(&sm.kv_empty[s], 2);  // both query tiles' products
+        mbar_init(&sm.kv_empty[s], 2 + (s & 1));  // both query tiles' products; for V (odd stages) the V-check warp
       }
-      mbar_init(&sm.v_go, 1);
       for (int i = 0; i < 3; ++i) mbar_init(&sm.v_clean[i], 1);
       mbar_init(&sm.next, 1);
       mbar_init(&sm.drain, 2);
@@ -286,16 +285,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
             float f[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(o[j]) * inv;
-            if (bad && live) {  // non-finite V that the row sees in the masked tiles
-              for (int key = w.i_mask * KT; key <= ti; ++key) {
-                const uint16_t* vr = p.v + (int64_t)(w.s0 + key) * p.v_st + w.h * p.v_sh + 32 * u;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  const float x = to_float<BF16>(vr[j]);
-                  if (!(fabsf(x) < INFINITY)) f[j] += x;
-                }
-              }
-            }
             // through shared memory, so that four lanes write 64 bytes of a row and a store meets 8 rows, not 32
             // (a row a lane: 5500 cycles for the tile's output, as long as one and a half key tiles)
 #pragma unroll
@@ -317,6 +306,21 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
               if (to >= 0) *reinterpret_cast<uint4*>(p.out + to * D + 32 * u + 8 * (lane & 3)) = x;
             }
             __syncwarp();
+          }
+          if (bad) {  // rare: non-finite V that the row sees in the masked tiles, over the finite part written above
+            __syncwarp();
+            if (live) {
+#pragma unroll 1
+              for (int c = 0; c < D; ++c) {
+                float sum = 0.0f;
+#pragma unroll 1
+                for (int key = w.i_mask * KT; key <= ti; ++key) {
+                  const float x = to_float<BF16>(p.v[(int64_t)(w.s0 + key) * p.v_st + w.h * p.v_sh + c]);
+                  if (!(fabsf(x) < INFINITY)) sum += x;
+                }
+                if (sum != 0.0f) p.out[row * D + c] = (uint16_t)pack2<BF16>(to_float<BF16>(p.out[row * D + c]) + sum, 0.0f);
+              }
+            }
           }
           if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m * p.c + log2f(l)) * kLn2;
           tc::fence_before();
@@ -348,8 +352,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
         tc::commit(&sm.s_full[q]);
         tc::commit(&sm.kv_empty[stage]);
       };
-      // checked tile m completes barrier m % 3. One query tile's warp may be two key tiles ahead of the other's, not
-      // three (the ring has STAGES < 6 stages), so neither warp meets a barrier one phase too early or too late
+      // checked tile m completes barrier m % 3. The check and either product warp are at most two key tiles apart, not
+      // three (the ring has STAGES < 6 stages), so no warp meets a barrier one phase too early or too late
       static_assert(STAGES < 6, "three barriers for checked tiles");
       auto v_clean = [&](int m) { return tc::wait_warp(&sm.v_clean[m % 3], (m / 3) & 1, abort); };
       auto full = [&](const Ring& r) { return tc::wait_warp(&sm.kv_full[r.stage], r.phase, abort); };
@@ -376,7 +380,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
           for (int i = 0; i < w.n && ok; ++i) {
             const bool more = i + 1 < w.n, check = i >= w.i_mask;
             ok = full(rv);
-            if (ok && check && q == 0 && lane == 0) tc::arrive(&sm.v_go);
             if (ok && more) ok = full(rk);
             if (ok && check) ok = v_clean(vc++);
             if (ok) ok = tc::wait_warp(&sm.p_half[q], pc & 1, abort);
@@ -496,18 +499,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
       }
       __syncwarp();
     } else {
-      // ---- V tiles with masked places: rows past the sequence and non-finite values to 0
-      int c = 0, vc = 0;
+      // ---- V tiles with masked places: rows past the sequence and non-finite values to 0. The warp sees every V tile
+      // as it lands (and gives back its hold on it), so the check is off the products' path.
+      static_assert(STAGES % 2 == 0, "V tiles on odd stages");
+      int vc = 0;
+      Ring rv = {1, 0};
       bool ok = true;
       for (int it = 0; ok; ++it) {
         ok = tc::wait_warp(&sm.item_full[it & 1], (it >> 1) & 1, abort);
         if (!ok || !w.read(sm.item[it & 1], TQ)) break;
-        for (int i = w.i_mask; i < w.n; ++i) {
-          const int cv = c + 2 * i + 1, s = cv % STAGES;
-          // a product warp says when the stage holds this tile: this warp sees
-          // only some of a stage's phases, so its parity alone could be an older one's
-          ok = tc::wait_warp(&sm.v_go, vc & 1, abort) && tc::wait_warp(&sm.kv_full[s], (cv / STAGES) & 1, abort);
+        for (int i = 0; i < w.n; ++i, rv.next()) {
+          const int s = rv.stage;
+          ok = tc::wait_warp(&sm.kv_full[s], rv.phase, abort);
           if (!ok) break;
+          if (i < w.i_mask) {
+            if (lane == 0) tc::arrive(&sm.kv_empty[s]);
+            continue;
+          }
           // chunk u: 16 bytes of row (u >> 3) & 127. x * 0 is NaN exactly for a value that is not finite, so a packed
           // multiply-add per pair looks at a chunk in four instructions (a test of each exponent took 4 us a tile)
           const int rows = min(KT, w.len - KT * i), first = lane;
@@ -541,10 +549,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
           if (found) sm.bad_v[it & 1] = 1u;
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) tc::arrive(&sm.v_clean[vc % 3]);
+          if (lane == 0) {
+            tc::arrive(&sm.v_clean[vc % 3]);
+            tc::arrive(&sm.kv_empty[s]);
+          }
           ++vc;
         }
-        c += 2 * w.n;
         __syncwarp();
         if (lane == 0) tc::arrive(&sm.item_empty[it & 1]);
       }

@@ -32,6 +32,13 @@ token attends causally to its sequence's packed tokens). vLLM must then be
 given at most the pool's block count (``num_gpu_blocks_override``); the
 kernels flag any block id past it.
 
+Two options, off by default: ``shared_prefix=True`` lets a decode batch that
+attends to every block (``top_k_blocks_decode=0``) and whose metadata names a
+common prefix (vLLM's ``common_prefix_len``) read that prefix once for the
+whole batch (fused.shared_prefix_decode); ``exact_prompts=True`` lets a batch of
+whole prompts, without the fp16 cache, attend to its own K and V before their
+quantisation (fused.prompt_attention) instead of reading them back from the pool.
+
 The base classes are vLLM's (``vllm.v1.attention.backends.flash_attn``);
 ``backend_cls`` / ``impl_cls`` may be passed to install against other
 classes with the same interface (the tests do).
@@ -56,6 +63,8 @@ _GQA: str = "mean"         # how the group's queries bound a page (the reference
 _LAYER_INDEX: dict[str, int] = {}
 _IMPL_CLS = None
 _FP16_CACHE: bool = True   # False: vLLM keeps no fp16 cache; prefill reads the pool
+_SHARED_PREFIX: bool = False  # decode batches on a common prefix read it once
+_EXACT_PROMPTS: bool = False  # whole prompts attend to their unquantised K and V
 
 
 def layer_index(layer) -> int | None:
@@ -126,6 +135,8 @@ def make_impl_cls(base):
                     raise NotImplementedError("the compact-pool backend without an fp16 cache supports causal "
                                               "decoder attention of the pool's layers only")
                 if getattr(attn_metadata, "max_query_len", 0) != 1:
+                    if _EXACT_PROMPTS and whole_prompts(attn_metadata, query, key):
+                        return prompts_into(query, key, value, attn_metadata, output, scale=float(self.scale))
                     return prefill_into(pool, idx, query, attn_metadata, output, scale=float(self.scale))
             elif passthrough:
                 return super().forward(layer, query, key, value, kv_cache, attn_metadata, output,
@@ -153,10 +164,46 @@ def decode_into(pool: CompactKVPool, idx: int, query: torch.Tensor, attn_metadat
     if _TOP_K > 0:
         sel = fused.quest_select(pool, idx, q, bt, seq_lens, top_k=_TOP_K, sink_pages=_SINK_BLOCKS, gqa=_GQA)
         o, _ = fused.decode(pool, idx, q, bt, seq_lens, sel, softmax_scale=scale, v_pos="physical")
+    elif _SHARED_PREFIX and B > 1 and common_prefix(attn_metadata, pool.block_size) > 0:
+        o, _ = fused.shared_prefix_decode(pool, idx, q, bt, seq_lens, common_prefix(attn_metadata, pool.block_size),
+                                          softmax_scale=scale, v_pos="physical")
     else:
         o, _ = fused.decode(pool, idx, q, bt, seq_lens, softmax_scale=scale, v_pos="physical")
     out = output[:n].view(B, Hq, D)
     out.copy_(o.to(out.dtype))
+    return output
+
+
+def common_prefix(attn_metadata, block_size: int) -> int:
+    """Tokens in whole blocks that every sequence of the batch shares, as vLLM's
+    metadata says (0 where it says nothing)."""
+    return int(getattr(attn_metadata, "common_prefix_len", 0) or 0) // block_size * block_size
+
+
+def whole_prompts(attn_metadata, query: torch.Tensor, key: torch.Tensor) -> bool:
+    """Whether every sequence of the batch is a whole prompt, as far as the
+    host can tell without reading the device: all chunks of the longest
+    chunk's length, and no sequence longer than that."""
+    n = int(getattr(attn_metadata, "num_actual_tokens", query.shape[0]))
+    B = int(attn_metadata.query_start_loc.shape[0]) - 1
+    longest = int(attn_metadata.max_query_len)
+    return (key is not None and query.shape[-1] in (64, 128) and query.dtype in (torch.float16, torch.bfloat16)
+            and key.dtype == query.dtype and n == B * longest
+            and int(getattr(attn_metadata, "max_seq_len", 0) or 0) == longest)
+
+
+def prompts_into(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, attn_metadata, output: torch.Tensor,
+                 scale: float) -> torch.Tensor:
+    """Whole prompts attend to their own K and V at full precision, into
+    ``output[:num_actual_tokens]``."""
+    n = int(getattr(attn_metadata, "num_actual_tokens", query.shape[0]))
+    Hq, D = query.shape[-2], query.shape[-1]
+    out = output[:n].view(n, Hq, D)
+    fits = out.dtype == query.dtype and out.is_contiguous()
+    o, _ = fused.prompt_attention(query[:n].reshape(n, Hq, D), key[:n].reshape(n, -1, D), value[:n].reshape(n, -1, D),
+                                  attn_metadata.query_start_loc, softmax_scale=scale, out=out if fits else None)
+    if not fits:
+        out.copy_(o.to(out.dtype))
     return output
 
 
@@ -201,15 +248,17 @@ def install_compact_backend(scales_path: str, *, num_layers: int = 28, num_block
                             block_size: int = 16, num_kv_heads: int = 4, head_size: int = 128,
                             device: str = "cuda:0", top_k_blocks_decode: int = 0, sink_blocks: int = 4,
                             gqa: str = "mean", scales: KVScales | None = None, backend_cls=None,
-                            impl_cls=None, fp16_cache: bool = True, attention_cls=None) -> None:
+                            impl_cls=None, fp16_cache: bool = True, attention_cls=None,
+                            shared_prefix: bool = False, exact_prompts: bool = False) -> None:
     """Allocate the compact pool and route vLLM's FlashAttention backend to
     ``KVQuantCompactImpl`` (compact_backend.py:70-119). Call before building
     the vLLM engine. ``top_k_blocks_decode`` = 0 attends to every block;
     ``scales`` (already loaded) takes the place of ``scales_path``.
     ``fp16_cache=False`` also removes vLLM's fp16 cache: ``attention_cls``
     (vLLM's Attention layer by default) reports the tiny KV-cache spec and
-    ``backend_cls`` the tiny shape; prefill then reads the compact pool."""
-    global _POOL, _SCALES, _TOP_K, _SINK_BLOCKS, _GQA, _IMPL_CLS, _FP16_CACHE
+    ``backend_cls`` the tiny shape; prefill then reads the compact pool.
+    ``shared_prefix`` and ``exact_prompts``: see the top of this module."""
+    global _POOL, _SCALES, _TOP_K, _SINK_BLOCKS, _GQA, _IMPL_CLS, _FP16_CACHE, _SHARED_PREFIX, _EXACT_PROMPTS
     if backend_cls is None or impl_cls is None:
         from vllm.v1.attention.backends.flash_attn import FlashAttentionBackend, FlashAttentionImpl
         backend_cls = backend_cls or FlashAttentionBackend
@@ -231,6 +280,8 @@ def install_compact_backend(scales_path: str, *, num_layers: int = 28, num_block
     _LAYER_INDEX.clear()
     _IMPL_CLS = make_impl_cls(impl_cls)
     _FP16_CACHE = bool(fp16_cache)
+    _SHARED_PREFIX = bool(shared_prefix)
+    _EXACT_PROMPTS = bool(exact_prompts)
     backend_cls.get_impl_cls = staticmethod(lambda: _IMPL_CLS)
     if not fp16_cache:
         backend_cls.get_kv_cache_shape = staticmethod(tiny_kv_cache_shape)

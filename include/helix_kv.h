@@ -145,7 +145,8 @@ HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_strid
  * once, when its last reference goes, in the order of the call's last entries
  * naming each freed page. *free_count_out = pages on the stack. A page without
  * a reference, an id outside [0, num_pages), bad lengths or a full stack are
- * HX_DEV_ERR_BOUNDS. One kernel. No reference counterpart.
+ * HX_DEV_ERR_BOUNDS. seq_lens_out and free_count_out must not overlap inputs.
+ * One kernel. No reference counterpart.
  */
 HX_API int hx_tables_truncate(void* stream, const int32_t* block_table, int64_t bt_stride, int32_t B,
                               int32_t max_pages, int32_t page_size, const int32_t* seq_lens,

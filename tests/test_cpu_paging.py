@@ -20,7 +20,8 @@ def test_entry_points_reject_bad_arguments_before_any_device_work():
     args[3] = 16385
     assert L.hx_tables_extend(*args) == hxlib.HX_ERR_UNSUPPORTED
     good = [None, one, 8, 1, 8, 16, one, one, one, 4, one, None, 4, two, two, None]
-    for i, bad in ((3, -1), (5, 0), (2, 7), (6, None), (7, None), (10, None), (13, None), (14, None), (12, -1)):
+    for i, bad in ((3, -1), (5, 0), (2, 7), (6, None), (7, None), (10, None), (13, None), (14, None), (12, -1), (13, one),
+                   (14, one)):
         args = list(good)
         args[i] = bad
         assert L.hx_tables_truncate(*args) == hxlib.HX_ERR_ARG, i

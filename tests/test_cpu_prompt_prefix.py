@@ -70,3 +70,66 @@ def test_shapes_and_types_are_refused():
                       ((q, k[..., :64], k[..., :64], s), ValueError)):
         with pytest.raises(err):
             fused.prompt_attention(*args)
+
+
+def _hook(monkeypatch, **state):
+    """The compact hook's module with recorders in place of the kernels."""
+    import types
+
+    from kvquant import compact_backend as cb
+    calls = []
+
+    def recorder(name, result):
+        def f(*args, **kw):
+            calls.append((name, args, kw))
+            return result(*args, **kw)
+        return f
+    half = lambda pool, li, q, *a, **kw: (torch.full(q.shape, 0.5), None)  # noqa: E731
+    prompt = lambda q, k, v, qs, out=None, **kw: (out.fill_(0.25) if out is not None else torch.full_like(q, 0.25), None)  # noqa: E731
+    monkeypatch.setattr(cb, "fused", types.SimpleNamespace(
+        decode=recorder("decode", half), shared_prefix_decode=recorder("shared", half),
+        prefill=recorder("prefill", half), prompt_attention=recorder("prompt", prompt)))
+    monkeypatch.setattr(cb, "_POOL", types.SimpleNamespace(num_layers=4, block_size=16))
+    monkeypatch.setattr(cb, "_TOP_K", 0)
+    for k, v in state.items():
+        monkeypatch.setattr(cb, k, v)
+    impl = cb.make_impl_cls(type("Base", (), {}))()
+    impl.scale, impl.sliding_window = 0.125, (-1, -1)
+    layer = types.SimpleNamespace(layer_name="model.layers.1.self_attn.attn")
+    return cb, impl, layer, calls
+
+
+def _meta(**kw):
+    import types
+    return types.SimpleNamespace(causal=True, **kw)
+
+
+def test_hook_decodes_a_shared_prefix_once_when_asked(monkeypatch):
+    bt, sl = torch.zeros((3, 9), dtype=torch.int32), torch.full((3,), 100, dtype=torch.int32)
+    q = torch.randn(4, 28, 128)
+    for asked, common, want in ((True, 70, "shared"), (True, 15, "decode"), (True, 0, "decode"), (False, 70, "decode")):
+        cb, impl, layer, calls = _hook(monkeypatch, _SHARED_PREFIX=asked)
+        out = torch.zeros(4, 28, 128, dtype=torch.float16)
+        impl.forward(layer, q, None, None, None, _meta(max_query_len=1, num_actual_tokens=3, block_table=bt, seq_lens=sl,
+                                                       common_prefix_len=common), out)
+        assert [c[0] for c in calls] == [want]
+        if want == "shared":
+            assert calls[0][1][5] == 64 and calls[0][2]["v_pos"] == "physical"  # whole blocks of the prefix
+        assert bool((out[:3] == 0.5).all()) and not out[3].any()
+
+
+def test_hook_attends_whole_prompts_exactly_when_asked(monkeypatch):
+    bt, q = torch.zeros((2, 9), dtype=torch.int32), torch.randn(12, 28, 128).half()
+    k = torch.randn(12, 4, 128).half()
+
+    def meta(n, longest, longest_seq):
+        return _meta(max_query_len=longest, max_seq_len=longest_seq, num_actual_tokens=n, block_table=bt,
+                     seq_lens=torch.tensor([5, 5]), query_start_loc=torch.tensor([0, 5, n]))
+    for asked, m, want in ((True, meta(10, 5, 5), "prompt"), (False, meta(10, 5, 5), "prefill"),
+                           (True, meta(10, 5, 9), "prefill"), (True, meta(9, 5, 5), "prefill")):
+        cb, impl, layer, calls = _hook(monkeypatch, _EXACT_PROMPTS=asked, _FP16_CACHE=False)
+        out = torch.zeros(12, 28, 128, dtype=torch.float16)
+        impl.forward(layer, q, k, k, None, m, out)
+        assert [c[0] for c in calls] == [want]
+        if want == "prompt":
+            assert bool((out[:10] == 0.25).all()) and not out[10:].any()
