@@ -43,7 +43,8 @@ struct Smem {
   alignas(256) uint32_t vpair[16];               // nuq2 V past t_cal: level pairs by code pair
   alignas(16) uint32_t vplane[8];                // nuq4 V past t_cal: byte planes
   alignas(16) uint8_t codes[2][PAGES][1024];     // each producer warp's next page (K, V)
-  uint64_t q_full[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], drain;
+  float2 ml[ROWS];                               // the second stream's (maximum, sum) of each row
+  uint64_t q_full[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], ml_full, ml_empty, drain;
   uint32_t tmem, abort;
 };
 
@@ -90,7 +91,7 @@ HX_DEVINL bool get_item(const Params& p, int j, int idx, Item& it) {
     it.page0 = ta * PAGES;
     it.pages = min(te * PAGES, p.prefix_pages) - it.page0;
     it.tokens = it.pages * S;
-    it.pidx = 2 * split;
+    it.pidx = split;
     it.trow = 0;
   } else {
     const int first = j - pre % p.J;
@@ -104,7 +105,7 @@ HX_DEVINL bool get_item(const Params& p, int j, int idx, Item& it) {
     it.tokens = len - p.prefix_pages * S;
     if (it.tokens < 0 || (len - 1) / S >= p.bt_stride) it.tokens = 0;  // the merge flags a bad length
     it.pages = (it.tokens + S - 1) / S;
-    it.pidx = 2 * p.n_splits;
+    it.pidx = p.n_splits;
     it.trow = (int64_t)b * p.bt_stride;
   }
   it.n = (it.pages + PAGES - 1) / PAGES;
@@ -153,10 +154,11 @@ HX_DEVINL uint4 lds128(uint32_t addr) {
 
 // ---- dequantisation: warp w's page of every tile, K (kv 0) or V (kv 1) operand.
 // A lane has 64 channels of one token. Its codes come a tile ahead by cp.async
-// into its own 32 bytes of shared memory (72 registers a thread do not hold
-// them as well: spilled, the kernel took 1.3 times as long), the page's list
-// record and table entry a tile ahead in registers, none of them looked at
-// before its turn (a look at load time waits for the load: 1.2 times).
+// into its own 32 bytes of shared memory: as second copies in registers they
+// were spilled (8 sequences on 1M tokens: 870 us against 513 at that step). The
+// page's list record and table entry come a tile ahead in registers, and none
+// is looked at before its turn, since a look at load time waits for the load
+// (753 against 644).
 template <int BITS, int KV, int SEG, int BASE>
 HX_DEVINL void produce(const Params& p, Smem& sm, int h, int j, int w) {
   const int lane = threadIdx.x & 31, t = lane >> 1, half = lane & 1;
@@ -322,6 +324,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int H = p.pool.num_kv_heads, G = p.G, TQ = p.TQ, Tc = p.sc.t_cal;
   const int h = blockIdx.x % H, j = blockIdx.x / H;
+  pdl_allow_next();  // the merge's CTAs fit beside this one's and wait for the whole grid
 
   if (warp == 24) {
     if (lane == 0) {
@@ -335,6 +338,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
         mbar_init(&sm.kv_full[s], PAGES);
         mbar_init(&sm.kv_empty[s], 1);
       }
+      mbar_init(&sm.ml_full, 4);
+      mbar_init(&sm.ml_empty, 4);
       mbar_init(&sm.drain, 1);
       sm.abort = 0u;
       fence_mbar_init();
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
     const int q = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t sb = tmem + lanes + 128 * q, ob = tmem + lanes + 256 + 128 * q;
-    int used = 0, done = 0;  // S tiles and O results of this warpgroup so far
+    int used = 0, done = 0, joined = 0;  // S tiles, O results and joined items of this warpgroup so far
     bool ok = true;
     for (int idx = 0; ok && get_item(p, j, idx, it); ++idx) {
       const int seq = it.seq0 + (it.two ? q * TQ : 0) + r / G;
@@ -468,32 +473,60 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
         if (lane == 0) tc::arrive(&sm.p_full[q]);
       }
       if (it.n == 0) continue;
-      // ---- the rows' partials
+      // ---- the rows' partials. The second stream's rows sit in the same TMEM lanes: the first warpgroup joins both
       if (ok && k > 0) ok = tc::wait_warp(&sm.o_full[q], done++ & 1, abort);
-      if (ok && any) {
+      if (!ok) break;
+      tc::fence_after();
+      if (!it.two && q == 1) {
+        sm.ml[r] = make_float2(m * p.c, l);  // -inf, 0 without a tile
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::arrive(&sm.ml_full);
+        ok = tc::wait_warp(&sm.ml_empty, joined++ & 1, abort);  // O may be overwritten
+        continue;
+      }
+      const int64_t rows = (int64_t)p.B * H * G;
+      const int64_t row = ((int64_t)(it.suffix ? it.seq0 : seq) * H + h) * G + (it.suffix ? r : r % G);
+      const int64_t at = (int64_t)it.pidx * rows + row;
+      float w0 = 1.0f, w1 = 0.0f, M = m * p.c;
+      bool both = false;
+      if (!it.two) {
+        ok = tc::wait_warp(&sm.ml_full, joined++ & 1, abort);
+        if (!ok) break;
         tc::fence_after();
-        const int64_t rows = (int64_t)p.B * H * G;
-        const int64_t row = ((int64_t)(it.suffix ? it.seq0 : seq) * H + h) * G + (it.suffix ? r : r % G);
-        const int64_t at = (int64_t)(it.pidx + (it.two ? 0 : q)) * rows + row;
-        if (live) p.part_ml[at] = make_float2(m * p.c, l);
-        if (k > 0) {
+        both = it.n > 1;
+        const float2 x = sm.ml[r];
+        const float top = fmaxf(M, x.x);
+        if (both && top != -INFINITY) {
+          w0 = tc::ex2(M - top);
+          w1 = tc::ex2(x.x - top);
+          M = top;
+          l = l * w0 + x.y * w1;
+        }
+      }
+      if (any) {
+        if (live) p.part_ml[at] = make_float2(M, l);
 #pragma unroll 1
-          for (int u = 0; u < D / 32; ++u) {
-            uint32_t o[32];
-            tc::ld32(o, ob + 32 * u);
-            tc::wait_ld();
-            if (live) {
-              uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + 32 * u);
+        for (int u = 0; u < D / 16; ++u) {
+          uint32_t o[16], o1[16];
+          tc::ld16(o, ob + 16 * u);
+          if (both) tc::ld16(o1, ob + 128 + 16 * u);
+          tc::wait_ld();
+          if (both) {
 #pragma unroll
-              for (int c = 0; c < 8; ++c) dst[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-            }
+            for (int c = 0; c < 16; ++c)
+              o[c] = __float_as_uint(__uint_as_float(o[c]) * w0 + __uint_as_float(o1[c]) * w1);
+          }
+          if (live) {
+            uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + 16 * u);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) dst[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
           }
         }
-        // a block of two tiles has one partial per split: the second place stays empty
-        if (it.two && live) p.part_ml[at + rows] = make_float2(-INFINITY, 0.0f);
-        tc::fence_before();
       }
+      tc::fence_before();
       __syncwarp();
+      if (!it.two && lane == 0) tc::arrive(&sm.ml_empty);
     }
   } else if (warp < 16) {
     produce<BK, 0, S * D * (BK + BV) / 8, 0>(p, sm, h, j, warp - 8);
@@ -640,7 +673,7 @@ __global__ void __launch_bounds__(32 * MW) merge_kernel(const MergeParams p) {
   const int b = (int)(row / p.Hq), len = p.seq_lens[b];
   // a padding row (no tokens), and one shorter than the prefix or past its table (flagged): nothing attended
   const bool bad = len != 0 && (len < p.prefix || (len - 1) / S >= p.bt_stride);
-  const int n = len == 0 || bad ? 0 : 2 * p.n_splits + (len > p.prefix ? 2 : 0);
+  const int n = len == 0 || bad ? 0 : p.n_splits + (len > p.prefix ? 1 : 0);
   if (bad && threadIdx.x == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float M = -INFINITY, l = 0.0f;
@@ -659,7 +692,7 @@ __global__ void __launch_bounds__(32 * MW) merge_kernel(const MergeParams p) {
 #pragma unroll 8
     for (int j = 0; j < cnt; ++j) {
       const float wj = __shfl_sync(0xffffffffu, wgt, j);
-      if (wj != 0.0f) {  // a place without a partial holds nothing
+      if (wj != 0.0f) {  // no weight: nothing to add (and nothing stored, where there were no keys)
         const float4 v = reinterpret_cast<const float4*>(p.part_o + ((int64_t)(i0 + j) * rows + row) * D)[lane];
         o.x += wj * v.x, o.y += wj * v.y, o.z += wj * v.z, o.w += wj * v.w;
       }
@@ -713,7 +746,7 @@ HX_API int32_t hx_prefix_splits(int32_t B, int32_t H, int32_t group, int32_t pre
 
 HX_API int64_t hx_prefix_scratch_bytes(int32_t B, int32_t H, int32_t group, int32_t n_splits) {
   if (B < 1 || H < 1 || group < 1 || n_splits < 0) return 0;
-  return (int64_t)(2 * n_splits + 2) * B * H * group * (px::D + 2) * 4;
+  return (int64_t)(n_splits + 1) * B * H * group * (px::D + 2) * 4;
 }
 
 HX_API int hx_prefix_decode(void* stream, const hx_pool_layer* pool, const hx_layer_scales* sc, const uint16_t* q,
@@ -754,7 +787,7 @@ HX_API int hx_prefix_decode(void* stream, const hx_pool_layer* pool, const hx_la
   p.n_splits = n_splits;
   p.vphys = (flags & HX_VPOS_PHYSICAL) ? 1 : 0;
   p.part_o = reinterpret_cast<float*>(scratch);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)(2 * n_splits + 2) * rows * px::D);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)(n_splits + 1) * rows * px::D);
   p.err = dev_err;
   // a CTA for each split of each row block and head, and more for the suffixes while SMs are left
   const int pre = p.RB * n_splits, wave = 148 / H > 1 ? 148 / H : 1;

@@ -85,6 +85,12 @@ HX_DEVINL void ld32(uint32_t* r, uint32_t addr) {
       : HX_R8(r, 0), HX_R8(r, 8), HX_R8(r, 16), HX_R8(r, 24)
       : "r"(addr));
 }
+HX_DEVINL void ld16(uint32_t* r, uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : HX_R8(r, 0), HX_R8(r, 8)
+      : "r"(addr));
+}
 HX_DEVINL void st32(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"

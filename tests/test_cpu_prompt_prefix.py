@@ -57,7 +57,7 @@ def test_prefix_decode_refuses_on_the_host():
         for pages in (1, 8, 9, 65536):
             n = L.hx_prefix_splits(B, 4, 7, pages)
             assert 1 <= n <= -(-pages // 8)
-            assert L.hx_prefix_scratch_bytes(B, 4, 7, n) == (2 * n + 2) * B * 28 * 130 * 4
+            assert L.hx_prefix_scratch_bytes(B, 4, 7, n) == (n + 1) * B * 28 * 130 * 4
 
 
 def test_shapes_and_types_are_refused():
