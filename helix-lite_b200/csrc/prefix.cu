@@ -22,6 +22,13 @@
 //   16-23  V dequantisation likewise: levels picked out of registers by prmt
 //          (each token's own row before t_cal, the last row after it)
 //   24     the query tiles and the matrix products (tcgen05.mma, one thread)
+//
+// What bounds it: at 8 sequences behind 1M tokens (nuq4, 409 us, 1.46 TB/s of
+// codes; fused.decode, which reads the prefix per sequence: 4,967) the
+// shared-memory pipe (59 % for table lookups, operand stores and waits, 24 %
+// more for the tensor core's operands) and issue slots (55 %) of 16
+// dequantising warps. At 64 sequences behind 32K (84 us) the softmax's two
+// passes and the 64 suffixes.
 #include "dequant.cuh"
 #include "tcgen.cuh"
 #include "tmap.cuh"
