@@ -250,3 +250,18 @@ def test_streams_graphs_and_repeats():
     assert torch.equal(outs[0][0], o2) and torch.equal(outs[0][1], l2)
     with pytest.raises(hxlib.HelixError, match="out of range"):   # sequence 2 now runs into table entries of -1
         gpu.check()
+
+
+def test_more_work_items_than_sms():
+    """Blocks of query rows past one wave of CTAs, and one KV head with a full
+    group of rows; a sample of the sequences is checked."""
+    from kvquant import fused
+    B, G, H = 700, 8, 8
+    suffixes = [i % 4 for i in range(B)]
+    gpu, orc, table = _build((4, 4), 48, suffixes, H=H, seed=40)
+    lens = [48 + s for s in suffixes]
+    q = _q(B, H * G, 41)
+    out, lse = fused.shared_prefix_decode(gpu, 0, q, _i32(table), _i32(lens), 48)
+    gpu.check()
+    keep = set(range(0, B, 37)) | {15, 16, 31, 32, B - 1}
+    _check(gpu, orc, table, lens, q, out, lse, 1 / math.sqrt(D), "logical", skip=set(range(B)) - keep)

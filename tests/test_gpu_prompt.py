@@ -227,3 +227,16 @@ def test_close_to_the_pool_prefill():
     b, _ = fused.prefill(pool, 0, q, qs, bt, torch.tensor([n], device="cuda"))
     pool.check()
     assert float((a.float() - b.float()).norm() / a.float().norm()) < 0.25
+
+
+def test_thousands_of_one_token_prompts():
+    """Each token sees itself alone: the output is its V, the lse its score."""
+    import hxlib
+    from kvquant import fused
+    n = 3001
+    q, k, v, start = _make([1] * n, 4, 2, 64, torch.float16, seed=31)
+    out, lse = fused.prompt_attention(q, k, v, torch.tensor(start, dtype=torch.int32, device="cuda"))
+    hxlib.check_device_errors()
+    assert torch.equal(out, v.repeat_interleave(2, 1))
+    s = (q.double() * k.double().repeat_interleave(2, 1)).sum(-1) / 8
+    assert bool(((lse.double() - s).abs() <= 2.0 ** -18 + s.abs() * 2.0 ** -22).all())
