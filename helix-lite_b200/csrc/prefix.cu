@@ -540,7 +540,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
   } else if (warp < 24) {
     produce<BV, 1, S * D * (BK + BV) / 8, S * D * BK / 8>(p, sm, h, j, warp - 16);
   } else {
-    if (warp == 24) {
     // ---- query tiles and matrix products
     constexpr uint32_t ids = tc::idesc_f16(0, ROWS, KT, 0), idv = tc::idesc_f16(0, ROWS, D, 1);
     int qn[2] = {0, 0}, used[2] = {0, 0};  // loads into a query buffer; S tiles of a warpgroup so far
@@ -649,7 +648,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
     if (tc::elect()) tc::commit(&sm.drain);  // and no product may be in flight when TMEM is freed
     __syncwarp();
     (void)mbar_wait(&sm.drain, 0);
-    }
   }
   tc::fence_before();
   __syncthreads();

@@ -44,7 +44,6 @@ constexpr int KT = 128;         // keys per tile
 constexpr int ROWS = 128;       // query rows per tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;  // P <= 2^8 before the maximum moves
-
 constexpr int kOutRow = 80;     // bytes of a staged output row: 64, and 16 so that eight rows meet all banks
 
 // A work item: two tiles of query rows of one (sequence, KV head).
@@ -59,8 +58,8 @@ struct Smem {
   alignas(16) uint8_t out[8][32 * kOutRow];  // 32 columns of a softmax warp's output rows
   alignas(16) uint32_t answer[2][4];         // next_cta
   Item item[2];
-  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], p_half[2], o_full[2], turn[2], v_clean[3];
-  uint64_t item_full[2], item_empty[2], next, drain;
+  uint64_t q_full[2], q_empty[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_half[2], p_full[2], o_full[2], turn[2];
+  uint64_t v_clean[3], item_full[2], item_empty[2], next, drain;
   uint32_t tmem, abort, bad_v[2];
 };
 
