@@ -12,8 +12,9 @@
 //           twice, on the even and on the odd key tiles
 //   suffix  (sequence): the sequence's own pages, its G rows alone, again as two
 //           streams of key tiles
-// Each leaves unnormalised partials (m, l, O) per row; a second kernel joins a
-// row's partials. Roles in a CTA (25 warps):
+// Each leaves unnormalised fp32 partials (m, l, O) per row; a second kernel joins
+// a row's partials. Scores, m and l are fp32; P is rounded to fp16 once, as the
+// matrix unit's operand (l keeps the unrounded values), and the output once. Roles in a CTA (25 warps):
 //   0-7    two softmax warpgroups, a row a thread (as in the prompt kernel: S
 //          and P in TMEM, the maximum moves only past 2^8)
 //   8-15   K dequantisation: warp w turns page w of each tile into 16 rows of the

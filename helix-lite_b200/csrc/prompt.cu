@@ -22,7 +22,7 @@
 // What bounds it: 20,011 tokens (fp16, 28 heads on 4) take 2,220 us, 1,293
 // TFLOP/s of unmasked products (cuBLAS 1,668 in a burst), at burst clocks and
 // 2,579 under the power cap (1,112; cuBLAS 1,395). A key tile's products are
-// 2,700 of its 3,300 cycles: those with both operands in shared memory run at
+// 2,700 of its about 3,500 cycles: those with both operands in shared memory run at
 // 106 cycles of 64; the rest is the part of a tile's softmax (exponentials on
 // the special-function unit: 1,024 cycles at least) that the other tile's
 // products do not cover.
