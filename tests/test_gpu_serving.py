@@ -107,3 +107,37 @@ def test_hook_options(monkeypatch):
     want, wl, mag = _formula(q, K, V, [0, n, 2 * n], 0.1)
     check_prompt(out[:2 * n], wl.float(), want, wl, mag, V, n, torch.ones(2 * n, dtype=torch.bool, device="cuda"))
     assert not out[2 * n:].any()
+
+
+def test_install_sets_the_options_and_defaults_leave_them_off():
+    import types
+
+    from kvquant import compact_backend as cb
+    from kvquant import fused
+    from kvquant.synthetic import NUQ4, make_kv, make_scales
+    sc = make_scales([NUQ4], H, D, t_cal=64, seed=2)
+    backend = type("Backend", (), {"get_impl_cls": None})
+    base = type("Impl", (), {"do_kv_cache_update": lambda self, *a: None})
+    kw = dict(num_layers=1, num_blocks=16, num_kv_heads=H, head_size=D, scales=sc, backend_cls=backend, impl_cls=base)
+    layer = types.SimpleNamespace(layer_name="model.layers.0.self_attn.attn")
+    K, V = make_kv(16 * S, H, D, seed=3, chan_seed=2)
+    slots = torch.arange(16 * S, device="cuda")
+    table = _i32([[0, 1, 2, 3], [0, 1, 4, 5]])
+    q = _q(2, H * G, 4)
+    meta = types.SimpleNamespace(max_query_len=1, num_actual_tokens=2, causal=True, block_table=table,
+                                 seq_lens=_i32([50, 40]), common_prefix_len=32)
+    got = {}
+    for asked in (True, False):
+        cb.install_compact_backend("", **kw, **({"shared_prefix": True, "exact_prompts": True} if asked else {}))
+        assert cb._SHARED_PREFIX is asked and cb._EXACT_PROMPTS is asked
+        impl = backend.get_impl_cls()()
+        impl.scale, impl.sliding_window = 0.1, (-1, -1)
+        impl.do_kv_cache_update(layer, K, V, None, slots)
+        out = torch.zeros((2, H * G, D), dtype=torch.float16, device="cuda")
+        impl.forward(layer, q, None, None, None, meta, out)
+        cb.pool().check()
+        if asked:
+            want, _ = fused.shared_prefix_decode(cb.pool(), 0, q, table, meta.seq_lens, 32, softmax_scale=0.1, v_pos="physical")
+        else:
+            want, _ = fused.decode(cb.pool(), 0, q, table, meta.seq_lens, softmax_scale=0.1, v_pos="physical")
+        assert torch.equal(out, want.half())
