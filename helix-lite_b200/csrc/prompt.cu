@@ -19,9 +19,9 @@
 // under the other's softmax. The products of a tile are issued in the order
 // PV(i), S(i + 1), so that S(i + 1) complete means O(i) complete.
 //
-// What bounds it: 20,011 tokens (fp16, 28 heads on 4) take 2,220 us, 1,293
+// What bounds it: 20,011 tokens (fp16, 28 heads on 4) take 2,190 us, 1,310
 // TFLOP/s of unmasked products (cuBLAS 1,668 in a burst), at burst clocks and
-// 2,579 under the power cap (1,112; cuBLAS 1,395). A key tile's products are
+// 2,535 under the power cap (1,132; cuBLAS 1,395). A key tile's products are
 // 2,700 of its about 3,500 cycles: those with both operands in shared memory run at
 // 106 cycles of 64; the rest is the part of a tile's softmax (exponentials on
 // the special-function unit: 1,024 cycles at least) that the other tile's
@@ -389,10 +389,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) prompt_kernel(const __grid_consta
             ok = full(rv);
             if (ok && more) ok = full(rk);
             if (ok && check) ok = v_clean(vc++);
-            if (ok) ok = tc::wait_warp(&sm.p_half[q], pc & 1, abort);
             // the tiles take turns, PV and S of one in a row: left to interleave, both finish together, both
-            // softmaxes run together, and the tensor core waits for them (4280 cycles a key tile)
+            // softmaxes run together, and the tensor core waits for them (4280 cycles a key tile). The turn comes before P
+            // as a rule, so P is waited for last (2%)
             if (ok && w.nq == 2) ok = tc::wait_warp(&sm.turn[q], turns++ & 1, abort);
+            if (ok) ok = tc::wait_warp(&sm.p_half[q], pc & 1, abort);
             if (ok && tc::elect()) {
               tc::fence_after();
               const uint32_t va = smem_u32(sm.kv[0]) + rv.stage * (KT * D * 2);
