@@ -32,20 +32,13 @@ DEV = "cuda"
 T_CAL = 4096
 
 
-_modules = None
-
-
 def _package():
-    """The framework's packages, as a program beside the repository imports them: once."""
-    global _modules
-    if _modules is not None:
-        return _modules
+    """The framework's packages, as a program beside the repository imports them."""
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "helix-lite_b200")
     if path not in sys.path:
         sys.path.insert(0, path)
     from kvquant import fused, paging
-    _modules = fused, paging
-    return _modules
+    return fused, paging
 
 
 # ---- cases ---------------------------------------------------------------------
