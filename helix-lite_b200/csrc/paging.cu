@@ -99,11 +99,15 @@ __global__ void __launch_bounds__(NT) extend_kernel(const ExtendParams p) {
   for (int b = b0; b < b1; ++b) {
     const long long c = p.cached[b], n = p.fresh[b];
     if (c < 0 || n < 0 || (c + n + p.S - 1) / p.S > p.W) {
-      mine = HX_DEV_ERR_BOUNDS;
+      mine |= HX_DEV_ERR_BOUNDS;
       continue;
     }
     st += n;
     sp += pages_of(c + n, p.S) - pages_of(c, p.S);
+    if (p.refs && n > 0 && c % p.S != 0) {  // the tokens begin in a page the sequence holds: nobody else may read it
+      const int page = p.table[b * p.stride + c / p.S];
+      if (page >= 0 && page < p.num_pages && p.refs[page] > 1) mine |= HX_DEV_ERR_SHARED;
+    }
   }
   long long it = st, ip = sp, tt, tp;
   block_scan2<NT>(it, ip, tt, tp, ws);

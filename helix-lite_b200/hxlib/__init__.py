@@ -19,7 +19,8 @@ LIB_PATH = Path(os.environ.get("HELIX_KV_LIB", _HERE / "libhelix_kv.so"))
 # status and device error bits (helix_kv.h)
 HX_OK, HX_ERR_ARG, HX_ERR_UNSUPPORTED, HX_ERR_LAUNCH, HX_ERR_SCRATCH_LIMIT = 0, 1, 2, 3, 4
 DEV_ERR = {0x1: "outlier arena full", 0x2: "index out of range", 0x4: "bounded wait ran out",
-           0x8: "selection threshold not isolated", 0x10: "too few free pages"}
+           0x8: "selection threshold not isolated", 0x10: "too few free pages",
+           0x20: "new tokens would fall into a shared page"}
 SEL_DENSE, SEL_THRESHOLD, SEL_LIST, SEL_SLICES = 0, 1, 2, 3
 VPOS_PHYSICAL = 0x100  # OR-ed into the decode's sel_mode (helix_kv.h)
 DECODE_CUDA_CORES = 0x200  # OR-ed into sel_mode: QK and PV in FFMA (helix_kv.h)

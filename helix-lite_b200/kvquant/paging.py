@@ -16,7 +16,8 @@ extended page starts at one reference, a truncated entry gives one back, and a
 page returns to the stack with its last reference. To share a prefix, copy
 table entries and add to the counts with torch (``block_table[rows, :n] =
 block_table[src, :n]``, ``page_refs[pages] += len(rows)``, cached length n *
-page_size); the pages past it are each sequence's own.
+page_size); the pages past it are each sequence's own. extend_tables refuses to
+write into a page of several references.
 
 Pages keep their statistics and outlier lists until they are emptied:
 ``CompactKVPool.reset_allocated`` empties, per layer, the pages that one
@@ -106,7 +107,11 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
     Too few free pages, a sequence past max_pages, more tokens than
     ``num_tokens`` or a negative length hand out nothing and flag a device
     error (CompactKVPool.check / hxlib.check_device_errors): all slots are -1
-    and seq_lens and free_count stay as they were.
+    and seq_lens and free_count stay as they were. With ``page_refs`` so does a
+    sequence whose new tokens would begin inside a page of more than one
+    reference (a shared prefix cut to a length inside a page): its other
+    holders read that page. Copy its rows to a page of the sequence's own
+    first, or cut to whole pages.
     """
     n_pages = _check(block_table, page_size, num_pages, free_pages, free_count, page_refs, cached_lens=cached_lens,
                      new_tokens=new_tokens)

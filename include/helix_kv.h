@@ -50,6 +50,7 @@ extern "C" {
 #define HX_DEV_ERR_TIMEOUT    0x4u  /* a bounded wait on a bulk copy ran out */
 #define HX_DEV_ERR_SELECT     0x8u  /* selection could not isolate a threshold */
 #define HX_DEV_ERR_PAGES      0x10u /* too few free pages for a batch's tables  */
+#define HX_DEV_ERR_SHARED     0x20u /* new tokens would fall into a shared page */
 
 /* Calibrated nuq scales of one layer (src/kvquant/scales.py:14-70). */
 typedef struct hx_layer_scales {
@@ -124,9 +125,12 @@ HX_API int hx_pool_reset_range(void* stream, const hx_pool_layer* pool, const in
  * tokens get slot -1 (hx_pack_append skips them) and position 0;
  * *free_count_out = pages left. Page ids must lie in [0, num_pages)
  * (HX_DEV_ERR_BOUNDS, slot -1). A negative length, a sequence past max_pages or
- * more than num_tokens tokens (HX_DEV_ERR_BOUNDS), or too few free pages
- * (HX_DEV_ERR_PAGES) hand out nothing: slots -1, query_start 0, seq_lens =
- * cached_lens, count unchanged. Outputs must not overlap inputs. One kernel.
+ * more than num_tokens tokens (HX_DEV_ERR_BOUNDS), too few free pages
+ * (HX_DEV_ERR_PAGES), or, with page_refs, a sequence whose new tokens would
+ * begin inside a page of more than one reference (HX_DEV_ERR_SHARED: others
+ * read that page; the sequence needs a copy of its own) hand out nothing: slots
+ * -1, query_start 0, seq_lens = cached_lens, count unchanged. Outputs must not
+ * overlap inputs. One kernel.
  * No reference counterpart (vLLM's scheduler builds these on the host).
  */
 HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_stride, int32_t B, int32_t max_pages,

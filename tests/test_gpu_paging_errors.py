@@ -1,0 +1,71 @@
+"""Table calls that cannot be served, or are given bad ids, counts and sizes:
+what they flag, and the tables, stack, counts and lengths they leave."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(v):
+    return torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")
+
+
+def _flagged(match):
+    import hxlib
+    with pytest.raises(hxlib.HelixError, match=match):
+        hxlib.check_device_errors()
+
+
+def _handed_out_nothing(out, table, was, cached, count, refs=None, refs_was=None):
+    assert torch.equal(table, was) and int(out.free_count) == count
+    assert bool((out.slot_mapping == -1).all()) and not out.query_start.any()
+    assert out.seq_lens.tolist() == list(cached)
+    if refs is not None:
+        assert torch.equal(refs, refs_was)
+
+
+# ---- a shared page is not written into
+
+@pytest.mark.parametrize("cut", [1, 5, 15])
+def test_extending_into_a_shared_page_hands_out_nothing(cut):
+    """Two sequences on one 3-page prefix; the second is cut inside the shared
+    third page. Its next tokens would fall into a page the first reads."""
+    from kvquant import paging
+    S, num = 16, 12
+    table = _i32([[4, 7, 2, 9, -1, -1], [4, 7, 2, 5, -1, -1]])
+    refs = torch.zeros(num, dtype=torch.int32, device="cuda")
+    refs[[4, 7, 2]] = 2
+    refs[[9, 5]] = 1
+    free, count = _i32([0, 1, 3, 6, 8, 10, 11, -1, -1, -1, -1, -1]), _i32([7])
+    lens, count = paging.truncate_tables(table, _i32([60, 60]), _i32([60, 3 * S - cut]), free, count, page_refs=refs)
+    assert lens.tolist() == [60, 48 - cut] and int(count) == 8
+    was, refs_was = table.clone(), refs.clone()
+    out = paging.extend_tables(table, lens, _i32([2, 3]), free, count, num_tokens=5, page_refs=refs)
+    _flagged("shared page")
+    _handed_out_nothing(out, table, was, lens.tolist(), 8, refs, refs_was)
+    # not extended, the same sequence stands in nobody's way
+    out = paging.extend_tables(table, lens, _i32([2, 0]), free, count, num_tokens=2, page_refs=refs)
+    import hxlib
+    hxlib.check_device_errors()
+    assert out.slot_mapping.tolist() == [9 * S + 12, 9 * S + 13]
+    # a page of its own (the caller copies the rows), and it goes on there
+    fresh = int(free[7])
+    table[1, 2] = fresh
+    refs[2] -= 1
+    refs[fresh] += 1
+    out = paging.extend_tables(table, lens, _i32([0, 3]), free, _i32([7]), num_tokens=3, page_refs=refs)
+    hxlib.check_device_errors()
+    assert out.slot_mapping.tolist()[0] == fresh * S + 16 - cut
+
+
+def test_whole_shared_pages_are_extended_past():
+    from kvquant import paging
+    import hxlib
+    table, refs = _i32([[3, 1, -1], [3, 1, -1]]), _i32([0, 2, 0, 2, 0])
+    out = paging.extend_tables(table, _i32([32, 32]), _i32([1, 16]), _i32([0, 2, 4]), _i32([3]), num_tokens=17, page_refs=refs)
+    hxlib.check_device_errors()
+    assert table.tolist() == [[3, 1, 4], [3, 1, 2]] and refs.tolist() == [0, 2, 1, 2, 1]
+    assert out.slot_mapping.tolist() == [64] + list(range(32, 48))
