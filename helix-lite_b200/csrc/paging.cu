@@ -10,9 +10,10 @@
 //
 // Both kernels are bound by launch latency except for large prompts, where
 // extend writes 16 bytes a token. So every CTA of extend repeats the scan over
-// the batch (B lengths from L2; no message between CTAs, one launch) and then
-// writes its own stretch of tokens and pages; page k comes straight from the
-// free stack, never from a table entry that another CTA writes. Truncate does
+// the batch and its checks (B lengths and every id to be popped, from L2; no
+// message between CTAs, one launch) and then writes its own stretch of tokens
+// and pages; page k comes straight from the free stack, never from a table
+// entry that another CTA writes. Truncate does
 // the same (giving back the 21,000 pages of 64 prompts: 9 us, against 19 with one
 // CTA), except with reference counts: shared pages need steps in order, which
 // one CTA takes.
@@ -104,14 +105,23 @@ __global__ void __launch_bounds__(NT) extend_kernel(const ExtendParams p) {
     }
     st += n;
     sp += pages_of(c + n, p.S) - pages_of(c, p.S);
-    if (p.refs && n > 0 && c % p.S != 0) {  // the tokens begin in a page the sequence holds: nobody else may read it
+    if (n > 0 && c % p.S != 0) {  // the tokens begin in a page the sequence holds: nobody else may read it
       const int page = p.table[b * p.stride + c / p.S];
-      if (page >= 0 && page < p.num_pages && p.refs[page] > 1) mine |= HX_DEV_ERR_SHARED;
+      if (page < 0 || page >= p.num_pages) mine |= HX_DEV_ERR_BOUNDS;
+      else if (p.refs && p.refs[page] > 1) mine |= HX_DEV_ERR_SHARED;
     }
   }
   long long it = st, ip = sp, tt, tp;
   block_scan2<NT>(it, ip, tt, tp, ws);
   const long long count = *p.free_count;
+  if (count >= 0 && count <= p.free_cap && tp <= count) {  // ids to be popped: all are looked at before any is handed out
+    const int n = (int)tp;
+#pragma unroll 4
+    for (int k = tid; k < n; k += NT) {
+      const int page = p.free_pages[count - 1 - k];
+      if (page < 0 || page >= p.num_pages) mine |= HX_DEV_ERR_BOUNDS;
+    }
+  }
   if (mine) atomicOr(&bad, mine);
   if (tid == 0) {
     if (tt > p.num_tokens || count < 0 || count > p.free_cap) atomicOr(&bad, HX_DEV_ERR_BOUNDS);
@@ -147,12 +157,8 @@ __global__ void __launch_bounds__(NT) extend_kernel(const ExtendParams p) {
     const int b = find_row(pf, p.B, k);
     const int j = pages_of(p.cached[b], p.S) + k - pf[b];
     const int page = p.free_pages[count - 1 - k];
-    if (page < 0 || page >= p.num_pages) {
-      set_err(p.err, HX_DEV_ERR_BOUNDS);
-      continue;
-    }
     p.table[(int64_t)b * p.stride + j] = page;
-    if (p.refs) p.refs[page] = 1;
+    if (p.refs && page >= 0 && page < p.num_pages) p.refs[page] = 1;  // (the stack may not change meanwhile)
   }
   // ---- tokens: slot and position; rows past the batch get slot -1 (skipped by the pack) and position 0
   for (int i = blockIdx.x * NT + tid; i < p.num_tokens; i += gridDim.x * NT) {
@@ -163,8 +169,7 @@ __global__ void __launch_bounds__(NT) extend_kernel(const ExtendParams p) {
       pos = (int64_t)c + i - qs[b];
       const int j = (int)(pos / p.S), have = pages_of(c, p.S);
       const int page = j < have ? p.table[(int64_t)b * p.stride + j] : p.free_pages[count - 1 - (pf[b] + j - have)];
-      if (page < 0 || page >= p.num_pages) set_err(p.err, HX_DEV_ERR_BOUNDS);
-      else slot = (int64_t)page * p.S + pos % p.S;
+      slot = (int64_t)page * p.S + pos % p.S;
     }
     p.slots[i] = slot;
     p.positions[i] = pos;

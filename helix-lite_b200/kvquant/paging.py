@@ -105,9 +105,11 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
     takes the results in existing tensors, which may not be the inputs.
 
     Too few free pages, a sequence past max_pages, more tokens than
-    ``num_tokens`` or a negative length hand out nothing and flag a device
-    error (CompactKVPool.check / hxlib.check_device_errors): all slots are -1
-    and seq_lens and free_count stay as they were. With ``page_refs`` so does a
+    ``num_tokens``, a negative length or a page id outside the pool (on the
+    stack among those to be popped, or in the table where a sequence goes on)
+    hand out nothing and flag a device error (CompactKVPool.check /
+    hxlib.check_device_errors): all slots are -1 and seq_lens and free_count
+    stay as they were. With ``page_refs`` so does a
     sequence whose new tokens would begin inside a page of more than one
     reference (a shared prefix cut to a length inside a page): its other
     holders read that page. Copy its rows to a page of the sequence's own

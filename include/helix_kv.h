@@ -123,9 +123,10 @@ HX_API int hx_pool_reset_range(void* stream, const hx_pool_layer* pool, const in
  * new_tokens), seq_lens = c + new, and for the num_tokens rows of the slot map
  * slot_mapping = page * S + position % S and positions; rows past the batch's
  * tokens get slot -1 (hx_pack_append skips them) and position 0;
- * *free_count_out = pages left. Page ids must lie in [0, num_pages)
- * (HX_DEV_ERR_BOUNDS, slot -1). A negative length, a sequence past max_pages or
- * more than num_tokens tokens (HX_DEV_ERR_BOUNDS), too few free pages
+ * *free_count_out = pages left. A negative length, a sequence past max_pages,
+ * more than num_tokens tokens, or an id outside [0, num_pages) among the pages
+ * to be popped or as the page that a sequence goes on filling
+ * (HX_DEV_ERR_BOUNDS), too few free pages
  * (HX_DEV_ERR_PAGES), or, with page_refs, a sequence whose new tokens would
  * begin inside a page of more than one reference (HX_DEV_ERR_SHARED: others
  * read that page; the sequence needs a copy of its own) hand out nothing: slots

@@ -69,3 +69,37 @@ def test_whole_shared_pages_are_extended_past():
     hxlib.check_device_errors()
     assert table.tolist() == [[3, 1, 4], [3, 1, 2]] and refs.tolist() == [0, 2, 1, 2, 1]
     assert out.slot_mapping.tolist() == [64] + list(range(32, 48))
+
+
+# ---- ids outside the pool
+
+@pytest.mark.parametrize("bad", [-1, 64, 2 ** 31 - 1, -2 ** 31])
+@pytest.mark.parametrize("counted", [False, True])
+@pytest.mark.parametrize("where", ["stack", "table"])
+def test_extend_with_a_bad_id_hands_out_nothing(bad, counted, where):
+    """On the stack among the pages to be popped, or as the page that a
+    sequence goes on filling: a row never ends up on a page it was not given."""
+    from kvquant import paging
+    rng = np.random.default_rng(3)
+    num, B, W = 64, 5, 8
+    perm = rng.permutation(num)
+    table = np.full((B, W), 33, np.int64)        # stale entries name a page that another may hold
+    cached = np.array([0, 5, 16, 31, 40])
+    at = 0
+    for b, c in enumerate(cached):
+        n = -(-c // 16)
+        table[b, :n] = perm[at:at + n]
+        at += n
+    refs = np.zeros(num, np.int64)
+    refs[perm[:at]] = 1
+    free = perm[at:].copy()
+    if where == "stack":
+        free[-7] = bad
+    else:
+        table[3, 1] = bad
+    g, gr, gf, count = _i32(table), _i32(refs) if counted else None, _i32(free), _i32([len(free)])
+    was, rw = g.clone(), gr.clone() if counted else None
+    out = paging.extend_tables(g, _i32(cached), _i32([20, 30, 40, 50, 10]), gf, count, num_tokens=160, page_refs=gr,
+                               num_pages=num)
+    _flagged("out of range")
+    _handed_out_nothing(out, g, was, cached, len(free), gr, rw)
