@@ -13,19 +13,26 @@
 // the batch and its checks (B lengths and every id to be popped, from L2; no
 // message between CTAs, one launch) and then writes its own stretch of tokens
 // and pages; page k comes straight from the free stack, never from a table
-// entry that another CTA writes. Truncate does
-// the same (giving back the 21,000 pages of 64 prompts: 9 us, against 19 with one
-// CTA), except with reference counts: shared pages need steps in order, which
-// one CTA takes.
+// entry that another CTA writes. Truncate runs as one cluster of up to 8 CTAs,
+// which agree through shared memory on whether an entry is bad before they push
+// any (giving back the 21,000 pages of 64 prompts: 10 us, against 19 with one
+// CTA; a million pages: 95 us); with reference counts shared pages need steps
+// in order, which one CTA takes.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace hx {
 namespace pg {
 
+namespace cg = cooperative_groups;
+
 constexpr int NT = 512;          // threads of a CTA of extend
 constexpr int NTT = 1024;        // threads of truncate's CTA
 constexpr int MAXB = 16384;      // sequences a call takes (their prefix sums sit in shared memory)
 constexpr int kTokensPerCta = 2048;
+constexpr int kCluster = 8;      // CTAs of truncate, at most
+constexpr int kHeld = 8;         // entries a thread of truncate holds in registers
 
 // Inclusive scan of (a, b) over the block's threads; totals to every thread.
 template <int N>
@@ -194,7 +201,8 @@ struct TruncateParams {
 
 // Drops pages [ceil(keep / S), ceil(len / S)) of every sequence. Dropped
 // entries are numbered k sequence by sequence and pushed in reverse, so that
-// truncating what extend just added leaves the stack as it was. With
+// truncating what extend just added leaves the stack as it was. An entry
+// outside the pool is an error and gives nothing back; the others do. With
 // reference counts an entry takes one reference; a page whose last reference
 // goes is pushed once, at the place of the call's last entry naming it (the
 // order does not depend on which thread's atomic came first):
@@ -205,11 +213,13 @@ struct TruncateParams {
 //   3  the entry that finds its own mark pushes the page; the mark becomes 0
 __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
   extern __shared__ int smem[];
-  int* pf = smem;
+  int* pf = smem;          // first dropped entry of each sequence
+  int* col = smem + p.B;   // table column of entry k: col + k
   __shared__ long long ws[NTT / 32][2];
   __shared__ uint32_t bad;
   __shared__ int freed, run;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const cg::cluster_group cluster = cg::this_cluster();  // the whole grid
   if (tid == 0) bad = 0u, freed = 0, run = 0;
   __syncthreads();
   const int per = (p.B + NTT - 1) / NTT, b0 = tid * per, b1 = min(p.B, b0 + per);
@@ -237,25 +247,83 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
     }
     return;
   }
+  if (gridDim.x > 1) cluster.barrier_arrive();  // this CTA's shared memory may be written
   int q = (int)(ip - sp);
   for (int b = b0; b < b1; ++b) {
+    const int kept = pages_of(max(0, min(p.keep[b], p.lens[b])), p.S);
     pf[b] = q;
-    q += pages_of(p.lens[b], p.S) - pages_of(max(0, min(p.keep[b], p.lens[b])), p.S);
+    col[b] = kept - q;
+    q += pages_of(p.lens[b], p.S) - kept;
   }
   __syncthreads();
   const int total = (int)tp;
-  auto entry = [&](int k) -> int {
-    const int b = find_row(pf, p.B, k);
-    const int j = pages_of(max(0, min(p.keep[b], p.lens[b])), p.S) + k - pf[b];
-    const int page = p.table[(int64_t)b * p.stride + j];
+  auto page_at = [&](int b, int k) -> int {  // entry k, of row b
+    const int page = p.table[(int64_t)b * p.stride + col[b] + k];
     if (page >= 0 && page < p.num_pages) return page;
     set_err(p.err, HX_DEV_ERR_BOUNDS);
     return -1;
   };
+  auto entry = [&](int k) { return page_at(find_row(pf, p.B, k), k); };
   constexpr int kMark = (int)0x80000000;
   if (!p.refs) {
-    for (int k = blockIdx.x * NTT + tid; k < total; k += gridDim.x * NTT) p.free_pages[count + total - 1 - k] = entry(k);
-    if (blockIdx.x != 0) return;
+    // a warp has a run of consecutive entries, so that a row is searched for once, not for every entry; the first
+    // pages of a lane stay in registers between the look at all entries and their push
+    const int warps = (int)gridDim.x * (NTT / 32), part = (total + 32 * warps - 1) / (32 * warps) * 32;
+    const int lo = min(total, ((int)blockIdx.x * (NTT / 32) + warp) * part), hi = min(total, lo + part);
+    int row = 0, first[kHeld];
+    auto next = [&](int k) {  // entry k, in the row of the lane's last entry or a later one
+      if (row + 1 < p.B && pf[row + 1] <= k) row = find_row(pf, p.B, k);
+      return page_at(row, k);
+    };
+    bool hole = false;  // an entry outside the pool
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const int k = lo + lane + 32 * u;
+      first[u] = k < hi ? next(k) : 0;
+      hole |= first[u] < 0;
+    }
+    for (int k = lo + lane + 32 * kHeld; k < hi; k += 32) hole |= next(k) < 0;
+    if (gridDim.x == 1) {
+      hole = __syncthreads_or(hole);
+    } else {  // every CTA is told
+      cluster.barrier_wait();
+      if (hole)
+        for (unsigned r = 0; r < gridDim.x; ++r) *cluster.map_shared_rank(&run, r) = 1;
+      cluster.sync();
+      hole = run != 0;
+    }
+    int good = total;
+    if (!hole) {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        const int k = lo + lane + 32 * u;
+        if (k < hi) p.free_pages[count + total - 1 - k] = first[u];
+      }
+      row = 0;
+      for (int k = lo + lane + 32 * kHeld; k < hi; k += 32) p.free_pages[count + total - 1 - k] = next(k);
+      if (blockIdx.x != 0) return;
+    } else {  // an error: one CTA pushes the good ones without a gap
+      if (blockIdx.x != 0) return;
+      good = 0;
+      for (int k0 = 0; k0 < total; k0 += NTT) good += __syncthreads_count(k0 + tid < total && entry(k0 + tid) >= 0);
+      int before = 0;
+      for (int k0 = 0; k0 < total; k0 += NTT) {
+        const int k = k0 + tid;
+        const int page = k < total ? entry(k) : -1;
+        const uint32_t m = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) ws[warp][0] = __popc(m);
+        __syncthreads();
+        int rank = before + __popc(m & ((1u << lane) - 1u));
+        for (int w = 0; w < NTT / 32; ++w) {
+          if (w < warp) rank += (int)ws[w][0];
+          before += (int)ws[w][0];
+        }
+        if (page >= 0) p.free_pages[count + good - 1 - rank] = page;
+        __syncthreads();
+      }
+    }
+    if (tid == 0) freed = good;
+    __syncthreads();
   } else {
     int here = 0;
     for (int k = tid; k < total; k += NTT) {
@@ -305,7 +373,7 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
     __syncthreads();
   }
   for (int b = tid; b < p.B; b += NTT) p.lens_out[b] = max(0, min(p.keep[b], p.lens[b]));
-  if (tid == 0) *p.free_out = (int32_t)(count + (p.refs ? freed : total));
+  if (tid == 0) *p.free_out = (int32_t)(count + freed);
 }
 
 // Empties pages[lo .. hi) (lo, hi read on the device) as hx_pool_reset_pages does.
@@ -381,16 +449,29 @@ HX_API int hx_tables_truncate(void* stream, const int32_t* block_table, int64_t 
   if (B > pg::MAXB) return HX_ERR_UNSUPPORTED;
   pg::TruncateParams p{block_table, bt_stride,  B,         max_pages, page_size,    seq_lens,       keep_lens, free_pages,
                        free_capacity, free_count, page_refs, num_pages, seq_lens_out, free_count_out, dev_err};
-  const size_t smem = (size_t)(B > 0 ? B : 1) * sizeof(int);
+  const size_t smem = (size_t)2 * (B > 0 ? B : 1) * sizeof(int);
   if (smem > 48 * 1024 && cudaFuncSetAttribute(pg::truncate_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)smem) != cudaSuccess) {
     (void)cudaGetLastError();
     return HX_ERR_LAUNCH;
   }
-  const int64_t most = page_refs ? 1 : ((int64_t)B * max_pages + 4 * pg::NTT - 1) / (4 * pg::NTT);  // entries, at most
-  const unsigned grid = most < 1 ? 1u : most > 148 ? 148u : (unsigned)most;
-  pg::truncate_kernel<<<grid, pg::NTT, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
-  HX_LAUNCH_CHECK();
+  // B * max_pages entries at most: more CTAs from two to a thread of one CTA
+  const unsigned grid = page_refs || (int64_t)B * max_pages <= 2 * pg::NTT ? 1u : (unsigned)pg::kCluster;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(pg::NTT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = grid;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = grid > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, pg::truncate_kernel, p) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return HX_ERR_LAUNCH;
+  }
   return HX_OK;
 }
 

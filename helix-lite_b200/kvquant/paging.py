@@ -157,8 +157,9 @@ def truncate_tables(block_table: torch.Tensor, seq_lens: torch.Tensor, keep_lens
     entry gives back one reference, and a page is pushed once, with its last
     reference, at the place of the call's last entry that names it. Table
     entries past the kept pages keep their old values. Returns (seq_lens,
-    free_count) as new tensors. A stack without room, or a page without a
-    reference to give back, flags a device error.
+    free_count) as new tensors. A page without a reference to give back, or an
+    entry outside the pool, flags a device error and gives nothing back; the
+    other entries do. A stack without room flags one as well.
     """
     n_pages = _check(block_table, page_size, num_pages, free_pages, free_count, page_refs, seq_lens=seq_lens,
                      keep_lens=keep_lens)

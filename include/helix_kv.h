@@ -149,8 +149,10 @@ HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_strid
  * stack. With page_refs an entry gives back one reference; a page is pushed
  * once, when its last reference goes, in the order of the call's last entries
  * naming each freed page. *free_count_out = pages on the stack. A page without
- * a reference, an id outside [0, num_pages), bad lengths or a full stack are
- * HX_DEV_ERR_BOUNDS. seq_lens_out and free_count_out must not overlap inputs.
+ * a reference or an id outside [0, num_pages) gives nothing back (the other
+ * entries do, N counting those alone); bad lengths, or without page_refs a full
+ * stack, give nothing back at all. All are HX_DEV_ERR_BOUNDS. seq_lens_out and
+ * free_count_out must not overlap inputs.
  * One kernel. No reference counterpart.
  */
 HX_API int hx_tables_truncate(void* stream, const int32_t* block_table, int64_t bt_stride, int32_t B,

@@ -103,3 +103,36 @@ def test_extend_with_a_bad_id_hands_out_nothing(bad, counted, where):
                                num_pages=num)
     _flagged("out of range")
     _handed_out_nothing(out, g, was, cached, len(free), gr, rw)
+
+
+@pytest.mark.parametrize("B,pages", [(4, 5), (64, 300)])
+@pytest.mark.parametrize("counted", [False, True])
+def test_truncate_gives_back_the_good_entries_only(B, pages, counted):
+    """Bad entries among those dropped: flagged, and neither pushed nor counted
+    (one CTA, and many)."""
+    from kvquant import paging
+    rng = np.random.default_rng(B)
+    num = B * pages + 10
+    perm = rng.permutation(num)
+    table = perm[:B * pages].reshape(B, pages).copy()
+    keep = rng.integers(0, pages * 16 + 1, B)
+    keep[0], keep[1] = 0, 7
+    bad = [(0, 0, -1), (0, pages - 1, num), (1, 1, 2 ** 31 - 1), (1, 0, -5)]   # the last one is kept, not dropped
+    for b, j, e in bad:
+        table[b, j] = e
+    refs = np.zeros(num, np.int64)
+    refs[table[(table >= 0) & (table < num)]] = 1
+    ent = [int(table[b, j]) for b in range(B) for j in range(-(-keep[b] // 16), pages)]
+    good = [p for p in ent if 0 <= p < num]
+    assert len(good) == len(ent) - 3
+    free = np.full(num, -1)
+    free[:10] = perm[-10:]
+    gf, gr = _i32(free), _i32(refs) if counted else None
+    lens, count = paging.truncate_tables(_i32(table), _i32([pages * 16] * B), _i32(keep), gf, _i32([10]), page_refs=gr,
+                                         num_pages=num)
+    _flagged("out of range")
+    assert int(count) == 10 + len(good) and lens.tolist() == keep.tolist()
+    assert gf[:int(count)].tolist() == free[:10].tolist() + good[::-1]
+    if counted:
+        refs[good] = 0
+        assert gr.tolist() == refs.tolist()
