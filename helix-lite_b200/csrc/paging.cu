@@ -16,7 +16,7 @@
 // entry that another CTA writes. Truncate runs as one cluster of up to 8 CTAs,
 // which agree through shared memory on whether an entry is bad before they push
 // any (giving back the 21,000 pages of 64 prompts: 10 us, against 19 with one
-// CTA; a million pages: 95 us); with reference counts shared pages need steps
+// CTA; a million pages: 68 us); with reference counts shared pages need steps
 // in order, which one CTA takes.
 #include <cooperative_groups.h>
 
@@ -32,7 +32,7 @@ constexpr int NTT = 1024;        // threads of truncate's CTA
 constexpr int MAXB = 16384;      // sequences a call takes (their prefix sums sit in shared memory)
 constexpr int kTokensPerCta = 2048;
 constexpr int kCluster = 8;      // CTAs of truncate, at most
-constexpr int kHeld = 8;         // entries a thread of truncate holds in registers
+constexpr int kHeld = 8;         // entries a thread of truncate holds in registers: a block of 256 a warp
 
 // Inclusive scan of (a, b) over the block's threads; totals to every thread.
 template <int N>
@@ -266,23 +266,30 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
   auto entry = [&](int k) { return page_at(find_row(pf, p.B, k), k); };
   constexpr int kMark = (int)0x80000000;
   if (!p.refs) {
-    // a warp has a run of consecutive entries, so that a row is searched for once, not for every entry; the first
-    // pages of a lane stay in registers between the look at all entries and their push
+    // a warp has a run of consecutive entries, so that a row is searched for once, not for every entry
     const int warps = (int)gridDim.x * (NTT / 32), part = (total + 32 * warps - 1) / (32 * warps) * 32;
     const int lo = min(total, ((int)blockIdx.x * (NTT / 32) + warp) * part), hi = min(total, lo + part);
-    int row = 0, first[kHeld];
-    auto next = [&](int k) {  // entry k, in the row of the lane's last entry or a later one
-      if (row + 1 < p.B && pf[row + 1] <= k) row = find_row(pf, p.B, k);
-      return page_at(row, k);
-    };
-    bool hole = false;  // an entry outside the pool
+    int row = 0, held[kHeld];
+    auto load = [&](int k0) {  // raw entries k0 + lane, + 32, ...: all on their way before one is looked at
 #pragma unroll
-    for (int u = 0; u < kHeld; ++u) {
-      const int k = lo + lane + 32 * u;
-      first[u] = k < hi ? next(k) : 0;
-      hole |= first[u] < 0;
+      for (int u = 0; u < kHeld; ++u) {
+        const int k = k0 + lane + 32 * u;
+        held[u] = 0;
+        if (k < hi) {
+          if (row + 1 < p.B && pf[row + 1] <= k) row = find_row(pf, p.B, k);
+          held[u] = p.table[(int64_t)row * p.stride + col[row] + k];
+        }
+      }
+    };
+    auto bad_id = [&](int page) { return page < 0 || page >= p.num_pages; };
+    bool hole = false;  // an entry outside the pool
+    int at = lo;
+    for (int k0 = lo; k0 < hi; k0 += 32 * kHeld) {
+      load(at = k0);
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) hole |= k0 + lane + 32 * u < hi && bad_id(held[u]);
     }
-    for (int k = lo + lane + 32 * kHeld; k < hi; k += 32) hole |= next(k) < 0;
+    if (hole) set_err(p.err, HX_DEV_ERR_BOUNDS);
     if (gridDim.x == 1) {
       hole = __syncthreads_or(hole);
     } else {  // every CTA is told
@@ -294,13 +301,17 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
     }
     int good = total;
     if (!hole) {
+      for (int k0 = at;;) {  // the last block of entries is still held, the others are loaded again
 #pragma unroll
-      for (int u = 0; u < kHeld; ++u) {
-        const int k = lo + lane + 32 * u;
-        if (k < hi) p.free_pages[count + total - 1 - k] = first[u];
+        for (int u = 0; u < kHeld; ++u) {
+          const int k = k0 + lane + 32 * u;
+          if (k < hi) p.free_pages[count + total - 1 - k] = held[u];
+        }
+        if (k0 == lo) break;
+        k0 -= 32 * kHeld;
+        row = 0;
+        load(k0);
       }
-      row = 0;
-      for (int k = lo + lane + 32 * kHeld; k < hi; k += 32) p.free_pages[count + total - 1 - k] = next(k);
       if (blockIdx.x != 0) return;
     } else {  // an error: one CTA pushes the good ones without a gap
       if (blockIdx.x != 0) return;
