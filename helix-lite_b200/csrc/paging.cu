@@ -31,6 +31,7 @@ constexpr int NT = 512;          // threads of a CTA of extend
 constexpr int NTT = 1024;        // threads of truncate's CTA
 constexpr int MAXB = 16384;      // sequences a call takes (their prefix sums sit in shared memory)
 constexpr int kTokensPerCta = 2048;
+constexpr int kMostDropped = (1 << 29) - 1;  // entries a truncate drops (their numbers mark pages, below 3 * -2^29)
 constexpr int kCluster = 8;      // CTAs of truncate, at most
 constexpr int kHeld = 8;         // entries a thread of truncate holds in registers: a block of 256 a warp
 
@@ -207,9 +208,13 @@ struct TruncateParams {
 // goes is pushed once, at the place of the call's last entry naming it (the
 // order does not depend on which thread's atomic came first):
 //   1  each entry takes a reference by compare-and-swap; the one that takes the
-//      last leaves INT_MIN in place of 0. An entry that finds no reference is
-//      an error and takes nothing
-//   2  entries of pages at INT_MIN raise it to INT_MIN + 1 + k (atomicMax)
+//      last leaves kGone in place of 0. An entry that comes later finds none:
+//      an error, counted by one less than kGone so that step 1 can be undone
+//      (each entry adds one again, which leaves kGone + the old count), as it
+//      is where the stack has no room for the pages freed. An entry of a page
+//      that had none is an error and changes nothing
+//   2  entries of pages at kGone or below lower it to INT_MIN + N - 1 - k
+//      (atomicMin: the last entry's mark stays)
 //   3  the entry that finds its own mark pushes the page; the mark becomes 0
 __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
   extern __shared__ int smem[];
@@ -234,7 +239,7 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
   block_scan2<NTT>(ip, dummy, tp, td, ws);
   const long long count = *p.free_count;
   if (mine) atomicOr(&bad, mine);
-  if (tid == 0 && (count < 0 || count > p.free_cap || tp > 0x7ffffff0ll || (!p.refs && count + tp > p.free_cap)))
+  if (tid == 0 && (count < 0 || count > p.free_cap || tp > kMostDropped || (!p.refs && count + tp > p.free_cap)))
     atomicOr(&bad, HX_DEV_ERR_BOUNDS);
   __syncthreads();
   if (bad) {  // nothing is given back
@@ -264,7 +269,8 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
     return -1;
   };
   auto entry = [&](int k) { return page_at(find_row(pf, p.B, k), k); };
-  constexpr int kMark = (int)0x80000000;
+  constexpr int kGone = -(1 << 30);
+  auto gone = [&](int refs) { return refs > kGone + kGone / 2 && refs < kGone / 2; };
   if (!p.refs) {
     // a warp has a run of consecutive entries, so that a row is searched for once, not for every entry
     const int warps = (int)gridDim.x * (NTT / 32), part = (total + 32 * warps - 1) / (32 * warps) * 32;
@@ -341,8 +347,8 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
       const int page = entry(k);
       if (page < 0) continue;
       int old = p.refs[page];
-      while (old > 0) {
-        const int seen = atomicCAS(p.refs + page, old, old == 1 ? kMark : old - 1);
+      while (old > 0 || gone(old)) {
+        const int seen = atomicCAS(p.refs + page, old, old == 1 ? kGone : old - 1);
         if (seen == old) break;
         old = seen;
       }
@@ -352,17 +358,36 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
     if (here) atomicAdd(&freed, here);
     __syncthreads();
     const int n_free = freed;
-    const bool fits = count + n_free <= p.free_cap;
-    if (!fits && tid == 0) set_err(p.err, HX_DEV_ERR_BOUNDS);
+    if (count + n_free > p.free_cap) {  // no room: every reference goes back, and nothing has happened
+      for (int k = tid; k < total; k += NTT) {
+        const int page = entry(k);
+        if (page < 0) continue;
+        const int now = __ldcg(p.refs + page);
+        if (now > 0 || gone(now)) atomicAdd(p.refs + page, 1);
+      }
+      __syncthreads();
+      for (int k = tid; k < total; k += NTT) {  // kGone + what there was
+        const int page = entry(k);
+        const int now = page < 0 ? 0 : __ldcg(p.refs + page);
+        if (gone(now)) atomicCAS(p.refs + page, now, now - kGone);
+      }
+      for (int b = tid; b < p.B; b += NTT) p.lens_out[b] = p.lens[b];
+      if (tid == 0) {
+        *p.free_out = (int32_t)count;
+        set_err(p.err, HX_DEV_ERR_BOUNDS);
+      }
+      return;
+    }
+    auto mark = [&](int k) { return (int)0x80000000 + (total - 1 - k); };  // below all that gone() takes
     for (int k = tid; k < total; k += NTT) {
       const int page = entry(k);
-      if (page >= 0 && __ldcg(p.refs + page) < 0) atomicMax(p.refs + page, kMark + 1 + k);
+      if (page >= 0 && __ldcg(p.refs + page) < kGone / 2) atomicMin(p.refs + page, mark(k));
     }
     __syncthreads();
     for (int k0 = 0; k0 < total; k0 += NTT) {  // ranks by a running block scan, chunk by chunk
       const int k = k0 + tid;
       const int page = k < total ? entry(k) : -1;
-      const bool mine_now = page >= 0 && __ldcg(p.refs + page) == kMark + 1 + k;
+      const bool mine_now = page >= 0 && __ldcg(p.refs + page) == mark(k);
       const uint32_t m = __ballot_sync(0xffffffffu, mine_now);
       if (lane == 0) ws[warp][0] = __popc(m);
       __syncthreads();
@@ -373,15 +398,13 @@ __global__ void __launch_bounds__(NTT) truncate_kernel(const TruncateParams p) {
       }
       if (mine_now) {
         const int rank = before + __popc(m & ((1u << lane) - 1u));
-        if (fits) p.free_pages[count + n_free - 1 - rank] = page;
+        if (rank < n_free) p.free_pages[count + n_free - 1 - rank] = page;  // (more: counts that were far below 0)
         p.refs[page] = 0;
       }
       __syncthreads();
       if (tid == 0) run += all;
       __syncthreads();
     }
-    if (!fits && tid == 0) freed = 0;
-    __syncthreads();
   }
   for (int b = tid; b < p.B; b += NTT) p.lens_out[b] = max(0, min(p.keep[b], p.lens[b]));
   if (tid == 0) *p.free_out = (int32_t)(count + freed);

@@ -159,7 +159,8 @@ def truncate_tables(block_table: torch.Tensor, seq_lens: torch.Tensor, keep_lens
     entries past the kept pages keep their old values. Returns (seq_lens,
     free_count) as new tensors. A page without a reference to give back, or an
     entry outside the pool, flags a device error and gives nothing back; the
-    other entries do. A stack without room flags one as well.
+    other entries do. A stack without room flags one as well, and then the
+    lengths, the counts and the stack stay as they were.
     """
     n_pages = _check(block_table, page_size, num_pages, free_pages, free_count, page_refs, seq_lens=seq_lens,
                      keep_lens=keep_lens)

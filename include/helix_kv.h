@@ -150,10 +150,11 @@ HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_strid
  * once, when its last reference goes, in the order of the call's last entries
  * naming each freed page. *free_count_out = pages on the stack. A page without
  * a reference or an id outside [0, num_pages) gives nothing back (the other
- * entries do, N counting those alone); bad lengths, or without page_refs a full
- * stack, give nothing back at all. All are HX_DEV_ERR_BOUNDS. seq_lens_out and
- * free_count_out must not overlap inputs.
- * One kernel. No reference counterpart.
+ * entries do, N counting those alone); bad lengths, a stack without room or
+ * more than 2^29 - 1 dropped entries give nothing back at all: seq_lens_out =
+ * seq_lens, counts and stack as they were. All are HX_DEV_ERR_BOUNDS.
+ * seq_lens_out and free_count_out must not overlap inputs. One kernel. No
+ * reference counterpart.
  */
 HX_API int hx_tables_truncate(void* stream, const int32_t* block_table, int64_t bt_stride, int32_t B,
                               int32_t max_pages, int32_t page_size, const int32_t* seq_lens,

@@ -136,3 +136,27 @@ def test_truncate_gives_back_the_good_entries_only(B, pages, counted):
     if counted:
         refs[good] = 0
         assert gr.tolist() == refs.tolist()
+
+
+# ---- a stack without room
+
+@pytest.mark.parametrize("twice", [False, True])
+def test_truncate_with_counts_onto_a_full_stack_gives_back_nothing(twice):
+    """Ten pages would come free (``twice``: nine, and some entries find no
+    reference to give back) on a stack with room for eight: counts, stack and
+    lengths stay as they were."""
+    from kvquant import paging
+    table = np.array([[3, 8, 5, 11], [3, 8, 5, 0], [3, 8, 2, 1], [13, 6, 4, 12]])
+    refs = np.zeros(14, np.int64)
+    for p in table.ravel():
+        refs[p] += 1
+    refs[3] = 5                                  # someone outside the batch holds it too
+    if twice:
+        refs[8], refs[5], refs[6] = 2, 1, 0      # fewer than the entries that name them
+    free = np.full(11, -1)
+    free[:3] = [7, 9, 10]
+    g, gf, gr = _i32(table), _i32(free), _i32(refs)
+    lens, count = paging.truncate_tables(g, _i32([64, 60, 50, 64]), _i32([0, 0, 0, 0]), gf, _i32([3]), page_refs=gr, num_pages=14)
+    _flagged("out of range")
+    assert gr.tolist() == refs.tolist() and gf.tolist() == free.tolist() and int(count) == 3
+    assert lens.tolist() == [64, 60, 50, 64]
