@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "tmap.cuh"
 
 namespace hx {
 namespace pg {
@@ -30,6 +31,7 @@ namespace cg = cooperative_groups;
 constexpr int NT = 512;          // threads of a CTA of extend
 constexpr int NTT = 1024;        // threads of truncate's CTA
 constexpr int MAXB = 16384;      // sequences a call takes (their prefix sums sit in shared memory)
+constexpr size_t kSmallSmem = 40 * 1024;  // dynamic shared memory asked for without more ado (48 KB with the static)
 constexpr int kTokensPerCta = 2048;
 constexpr int kMostDropped = (1 << 29) - 1;  // entries a truncate drops (their numbers mark pages, below 3 * -2^29)
 constexpr int kCluster = 8;      // CTAs of truncate, at most
@@ -459,11 +461,8 @@ HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_strid
                      free_pages,  free_capacity, free_count, page_refs, num_pages, query_start, seq_lens,
                      slot_mapping, positions,   num_tokens, free_count_out, dev_err};
   const size_t smem = (size_t)2 * (B > 0 ? B : 1) * sizeof(int);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(pg::extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return HX_ERR_LAUNCH;
-  }
+  static unsigned long long done = 0;
+  if (smem > pg::kSmallSmem && !allow_smem(pg::extend_kernel, 2 * pg::MAXB * (int)sizeof(int), done)) return HX_ERR_LAUNCH;
   int grid = (num_tokens + pg::kTokensPerCta - 1) / pg::kTokensPerCta;
   grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
   pg::extend_kernel<<<grid, pg::NT, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
@@ -484,11 +483,8 @@ HX_API int hx_tables_truncate(void* stream, const int32_t* block_table, int64_t 
   pg::TruncateParams p{block_table, bt_stride,  B,         max_pages, page_size,    seq_lens,       keep_lens, free_pages,
                        free_capacity, free_count, page_refs, num_pages, seq_lens_out, free_count_out, dev_err};
   const size_t smem = (size_t)2 * (B > 0 ? B : 1) * sizeof(int);
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(pg::truncate_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)smem) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return HX_ERR_LAUNCH;
-  }
+  static unsigned long long done = 0;
+  if (smem > pg::kSmallSmem && !allow_smem(pg::truncate_kernel, 2 * pg::MAXB * (int)sizeof(int), done)) return HX_ERR_LAUNCH;
   // B * max_pages entries at most: more CTAs from two to a thread of one CTA
   const unsigned grid = page_refs || (int64_t)B * max_pages <= 2 * pg::NTT ? 1u : (unsigned)pg::kCluster;
   cudaLaunchConfig_t cfg = {};

@@ -2,6 +2,10 @@
 what they flag, and the tables, stack, counts and lengths they leave."""
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -160,3 +164,29 @@ def test_truncate_with_counts_onto_a_full_stack_gives_back_nothing(twice):
     _flagged("out of range")
     assert gr.tolist() == refs.tolist() and gf.tolist() == free.tolist() and int(count) == 3
     assert lens.tolist() == [64, 60, 50, 64]
+
+
+# ---- batch sizes whose lengths just fill the default shared memory
+
+@pytest.mark.parametrize("call,B", [("extend", 6112), ("extend", 6144), ("truncate", 6112), ("truncate", 6144)])
+def test_batches_around_the_default_shared_memory(call, B):
+    """In a process of its own: a larger batch raises the kernel's limit for good."""
+    code = f"""
+import torch, hxlib
+from kvquant import paging
+B = {B}
+z = lambda n: torch.zeros(n, dtype=torch.int32, device="cuda")
+t, f = z((B, 1)), torch.arange(B, dtype=torch.int32, device="cuda")
+if "{call}" == "extend":
+    r = paging.extend_tables(t, z(B), z(B) + 1, f, z(1) + B, num_tokens=B)
+    hxlib.check_device_errors()
+    assert int(r.free_count) == 0 and torch.equal(r.slot_mapping, torch.arange(B - 1, -1, -1, device="cuda") * 16)
+else:
+    t[:, 0] = f
+    lens, count = paging.truncate_tables(t, z(B) + 9, z(B), z(B), z(1))
+    hxlib.check_device_errors()
+    assert int(count) == B and not lens.any()
+"""
+    root = Path(__file__).resolve().parents[1] / "helix-lite_b200"
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
