@@ -32,6 +32,7 @@ constexpr int NT = 512;          // threads of a CTA of extend
 constexpr int NTT = 1024;        // threads of truncate's CTA
 constexpr int MAXB = 16384;      // sequences a call takes (their prefix sums sit in shared memory)
 constexpr size_t kSmallSmem = 40 * 1024;  // dynamic shared memory asked for without more ado (48 KB with the static)
+constexpr int kMostRows = 1 << 30;  // tokens, and new pages, of an extend: a thread's next one still fits 32 bits
 constexpr int kTokensPerCta = 2048;
 constexpr int kMostDropped = (1 << 29) - 1;  // entries a truncate drops (their numbers mark pages, below 3 * -2^29)
 constexpr int kCluster = 8;      // CTAs of truncate, at most
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(NT) extend_kernel(const ExtendParams p) {
   uint32_t mine = 0u;
   for (int b = b0; b < b1; ++b) {
     const long long c = p.cached[b], n = p.fresh[b];
-    if (c < 0 || n < 0 || (c + n + p.S - 1) / p.S > p.W) {
+    if (c < 0 || n < 0 || c + n > 0x7fffffffll || (c + n + p.S - 1) / p.S > p.W) {
       mine |= HX_DEV_ERR_BOUNDS;
       continue;
     }
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(NT) extend_kernel(const ExtendParams p) {
   long long it = st, ip = sp, tt, tp;
   block_scan2<NT>(it, ip, tt, tp, ws);
   const long long count = *p.free_count;
-  if (count >= 0 && count <= p.free_cap && tp <= count) {  // ids to be popped: all are looked at before any is handed out
+  if (count >= 0 && count <= p.free_cap && tp <= count && tp <= kMostRows) {  // ids to be popped: all are looked at before any is handed out
     const int n = (int)tp;
 #pragma unroll 4
     for (int k = tid; k < n; k += NT) {
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(NT) extend_kernel(const ExtendParams p) {
   }
   if (mine) atomicOr(&bad, mine);
   if (tid == 0) {
-    if (tt > p.num_tokens || count < 0 || count > p.free_cap) atomicOr(&bad, HX_DEV_ERR_BOUNDS);
+    if (tt > p.num_tokens || count < 0 || count > p.free_cap || tp > kMostRows) atomicOr(&bad, HX_DEV_ERR_BOUNDS);
     else if (tp > count) atomicOr(&bad, HX_DEV_ERR_PAGES);
   }
   __syncthreads();
@@ -456,7 +457,7 @@ HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_strid
   if (B > 0 && (!block_table || !cached_lens || !new_tokens || !seq_lens || bt_stride < max_pages)) return HX_ERR_ARG;
   if (B > 0 && (seq_lens == cached_lens || seq_lens == new_tokens)) return HX_ERR_ARG;
   if ((num_tokens > 0 && (!slot_mapping || !positions)) || (free_capacity > 0 && !free_pages)) return HX_ERR_ARG;
-  if (B > pg::MAXB) return HX_ERR_UNSUPPORTED;
+  if (B > pg::MAXB || num_tokens > pg::kMostRows) return HX_ERR_UNSUPPORTED;
   pg::ExtendParams p{block_table, bt_stride,   B,        max_pages,   page_size, cached_lens,  new_tokens,
                      free_pages,  free_capacity, free_count, page_refs, num_pages, query_start, seq_lens,
                      slot_mapping, positions,   num_tokens, free_count_out, dev_err};

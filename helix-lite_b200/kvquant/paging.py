@@ -71,8 +71,8 @@ def _check(block_table, page_size, num_pages, free_pages, free_count, page_refs,
         raise ValueError("block_table rows must be contiguous and must not overlap")
     if free_count.shape[0] != 1:
         raise ValueError("free_count should be one number")
-    if page_size < 1:
-        raise ValueError("page_size must be at least 1")
+    if not 1 <= page_size < 1 << 31:
+        raise ValueError("page_size must be at least 1 and fit 32 bits")
     n = int(num_pages) if num_pages is not None else (page_refs if page_refs is not None else free_pages).shape[0]
     if page_refs is not None and page_refs.shape[0] < n:
         raise ValueError(f"page_refs should hold one count for each of {n} pages")
@@ -120,8 +120,8 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
     B, W = block_table.shape
     dev = block_table.device
     T = int(num_tokens)
-    if T < 0:
-        raise ValueError("num_tokens must not be negative")
+    if not 0 <= T <= 1 << 30:
+        raise ValueError(f"num_tokens must lie in 0 .. 2^30, got {T}")
     if out is None:
         i32, i64 = free_count.new_empty, torch.int64
         out = BatchTables(i32(B + 1), i32(B), i32(T, dtype=i64), i32(T, dtype=i64), i32(1))

@@ -114,24 +114,27 @@ HX_API int hx_pool_reset_range(void* stream, const hx_pool_layer* pool, const in
 /* ---- block tables and slot maps --------------------------------------- */
 
 /*
- * Room for new_tokens[b] more tokens in each of B sequences (at most 16384).
- * A sequence of c = cached_lens[b] tokens holds table entries [0, ceil(c / S))
- * of row block_table + b * bt_stride (max_pages entries) and gets those up to
- * ceil((c + new) / S): the k-th new page of the call, sequence by sequence, is
+ * Room for new_tokens[b] more tokens in each of B sequences (at most 16384; at
+ * most 2^30 tokens and 2^30 new pages in a call). A sequence of c =
+ * cached_lens[b] tokens holds table entries [0, ceil(c / S)) of row block_table
+ * + b * bt_stride (max_pages entries) and gets those up to ceil((c + new) / S):
+ * the k-th new page of the call, sequence by sequence, is
  * free_pages[*free_count - 1 - k]. Writes those entries, page_refs[page] = 1
  * for each (when non-NULL), query_start (B + 1, exclusive prefix of
  * new_tokens), seq_lens = c + new, and for the num_tokens rows of the slot map
  * slot_mapping = page * S + position % S and positions; rows past the batch's
  * tokens get slot -1 (hx_pack_append skips them) and position 0;
- * *free_count_out = pages left. A negative length, a sequence past max_pages,
- * more than num_tokens tokens, or an id outside [0, num_pages) among the pages
- * to be popped or as the page that a sequence goes on filling
- * (HX_DEV_ERR_BOUNDS), too few free pages
- * (HX_DEV_ERR_PAGES), or, with page_refs, a sequence whose new tokens would
- * begin inside a page of more than one reference (HX_DEV_ERR_SHARED: others
- * read that page; the sequence needs a copy of its own) hand out nothing: slots
- * -1, query_start 0, seq_lens = cached_lens, count unchanged. Outputs must not
- * overlap inputs. One kernel.
+ * *free_count_out = pages left. Some calls hand out nothing (slots -1,
+ * query_start 0, seq_lens = cached_lens, count unchanged):
+ *   HX_DEV_ERR_BOUNDS  a negative length, a sequence past max_pages or 2^31 - 1
+ *                      tokens, more than num_tokens tokens, or an id outside
+ *                      [0, num_pages) among the pages to be popped or as the
+ *                      page that a sequence goes on filling
+ *   HX_DEV_ERR_PAGES   too few free pages
+ *   HX_DEV_ERR_SHARED  with page_refs, a sequence whose new tokens would begin
+ *                      inside a page of more than one reference: others read
+ *                      that page, the sequence needs a copy of its own
+ * Outputs must not overlap inputs. One kernel.
  * No reference counterpart (vLLM's scheduler builds these on the host).
  */
 HX_API int hx_tables_extend(void* stream, int32_t* block_table, int64_t bt_stride, int32_t B, int32_t max_pages,

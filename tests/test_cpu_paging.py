@@ -38,3 +38,13 @@ def test_cpu_tensors_are_refused():
         paging.truncate_tables(t, v, v, v, v[:1])
     with pytest.raises(ValueError):
         paging.extend_tables(v, v, v, v, v[:1], num_tokens=1)
+
+
+def test_sizes_past_what_a_call_counts_are_refused():
+    """A thread's token and page numbers stay in 32 bits up to 2^30 of them."""
+    L = hxlib.lib()
+    one, two = hxlib.ctypes.c_void_p(256), hxlib.ctypes.c_void_p(512)   # never read
+    args = [None, one, 8, 1, 8, 16, one, one, one, 4, one, None, 4, two, two, two, two, (1 << 30) + 1, two, None]
+    assert L.hx_tables_extend(*args) == hxlib.HX_ERR_UNSUPPORTED
+    args[17] = 2 ** 31 - 1
+    assert L.hx_tables_extend(*args) == hxlib.HX_ERR_UNSUPPORTED

@@ -190,3 +190,26 @@ else:
     root = Path(__file__).resolve().parents[1] / "helix-lite_b200"
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ---- lengths at the border of 32 bits
+
+def test_lengths_past_32_bits_are_refused():
+    from kvquant import paging
+    import hxlib
+    S = 1 << 20
+    table = torch.arange(2049, dtype=torch.int32, device="cuda")[None].contiguous()
+    free, was = _i32([2049, 2050]), table.clone()
+    for new, fits in ((8, False), (7, True)):
+        out = paging.extend_tables(table, _i32([2 ** 31 - 8]), _i32([new]), free, _i32([2]), num_tokens=8, page_size=S,
+                                   num_pages=3000)
+        if fits:
+            hxlib.check_device_errors()
+            assert out.seq_lens.tolist() == [2 ** 31 - 1]
+            assert out.slot_mapping.tolist() == [2047 * S + S - 8 + i for i in range(7)] + [-1]
+        else:
+            _flagged("out of range")
+            _handed_out_nothing(out, table, was, [2 ** 31 - 8], 2)
+    for kw in (dict(num_tokens=2 ** 30 + 1), dict(num_tokens=2 ** 32 + 8), dict(num_tokens=8, page_size=2 ** 32 + 16)):
+        with pytest.raises(ValueError):
+            paging.extend_tables(table, _i32([0]), _i32([8]), free, _i32([2]), **kw)
