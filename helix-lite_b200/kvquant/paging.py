@@ -83,6 +83,12 @@ _I32 = torch.int32
 _SIZED = ("free_pages", "free_count", "page_refs")
 
 
+def _span(t):
+    """Addresses that a tensor reaches over: first byte, and the one past the last."""
+    lo = t.data_ptr()
+    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _row_stride(block_table):
     B, W = block_table.shape
     return int(block_table.stride(0)) if B > 1 else W
@@ -102,7 +108,8 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
     (the pool's block count; default: the length of page_refs or free_pages)
     bounds the page ids. Inputs other than block_table and page_refs are not
     changed: carry ``seq_lens`` and ``free_count`` on to the next step. ``out``
-    takes the results in existing tensors, which may not be the inputs.
+    takes the results in existing tensors, which may overlap neither the inputs
+    nor each other.
 
     Too few free pages, a sequence past max_pages, more tokens than
     ``num_tokens``, a negative length or a page id outside the pool (on the
@@ -126,7 +133,8 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
         i32, i64 = free_count.new_empty, torch.int64
         out = BatchTables(i32(B + 1), i32(B), i32(T, dtype=i64), i32(T, dtype=i64), i32(1))
     else:
-        ins = {t.data_ptr() for t in (cached_lens, new_tokens, free_count, free_pages, block_table) if t.numel()}
+        taken = [(_span(t), "one of the inputs") for t in (cached_lens, new_tokens, free_count, free_pages, block_table,
+                                                           page_refs) if t is not None and t.numel()]
         for name, n, dt in (("query_start", B + 1, torch.int32), ("seq_lens", B, torch.int32),
                             ("slot_mapping", T, torch.int64), ("positions", T, torch.int64),
                             ("free_count", 1, torch.int32)):
@@ -134,8 +142,12 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
             hxlib.require_cuda(t)
             if t.shape != (n,) or t.dtype != dt or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"out.{name} must be a contiguous ({n},) {dt} tensor on {dev}")
-            if n and t.data_ptr() in ins:
-                raise ValueError(f"out.{name} must not be one of the inputs")
+            if n:
+                lo, hi = _span(t)
+                for (a, e), whose in taken:
+                    if lo < e and a < hi:
+                        raise ValueError(f"out.{name} must not overlap {whose}")
+                taken.append(((lo, hi), f"out.{name}"))
     i = dev.index
     with hxlib.on(i):
         call("hx_tables_extend", hxlib.raw_stream(i), block_table.data_ptr(), _row_stride(block_table), B, W,

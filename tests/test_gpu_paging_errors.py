@@ -213,3 +213,27 @@ def test_lengths_past_32_bits_are_refused():
     for kw in (dict(num_tokens=2 ** 30 + 1), dict(num_tokens=2 ** 32 + 8), dict(num_tokens=8, page_size=2 ** 32 + 16)):
         with pytest.raises(ValueError):
             paging.extend_tables(table, _i32([0]), _i32([8]), free, _i32([2]), **kw)
+
+
+# ---- results in tensors that another argument or result also names
+
+def test_outputs_that_alias_are_refused():
+    from kvquant import paging
+    table, cached, new = _i32([[-1, -1]]), _i32([0]), _i32([3])
+    free, count, refs = _i32([0, 1, 2]), _i32([3]), _i32([0, 0, 0])
+
+    def out(**kw):
+        o = paging.BatchTables(_i32([0, 0]), _i32([0]), torch.zeros(3, dtype=torch.int64, device="cuda"),
+                               torch.zeros(3, dtype=torch.int64, device="cuda"), _i32([0]))
+        for k, t in kw.items():
+            setattr(o, k, t)
+        return o
+    one = _i32([0])
+    long = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for kw in (dict(free_count=one, seq_lens=one), dict(seq_lens=refs[1:2]), dict(free_count=free[2:]),
+               dict(query_start=refs[1:]), dict(slot_mapping=long[1:], positions=long[:3])):
+        with pytest.raises(ValueError, match="out"):
+            paging.extend_tables(table, cached, new, free, count, num_tokens=3, page_refs=refs, out=out(**kw))
+    ok = paging.extend_tables(table, cached, new, free, count, num_tokens=3, page_refs=refs,
+                              out=out(slot_mapping=torch.cat([long, long])[:3], query_start=_i32([0, 0, 0, 0])[1:3]))
+    assert ok.slot_mapping.tolist() == [32, 33, 34] and ok.seq_lens.tolist() == [3]
