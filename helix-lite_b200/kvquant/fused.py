@@ -434,7 +434,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     prompt's tokens up to itself. The three may be slices of one projection
     (last dimension contiguous, strides of 16 bytes; other layouts are
     copied). Returns (out (T, Hq, D) in the input type, lse (T, Hq) fp32 natural
-    log); rows past the last prompt are not written. ``prefill`` is the same
+    log); rows past the last prompt are not written. ``out`` may be ``query``
+    itself, and overlaps no other input. ``prefill`` is the same
     attention read back from the pool's quantised pages; here the prompt's own
     K and V, before write_kv packs them, give the unquantised result. K and V
     are read as they are (infinities and NaN of tokens that a row does not see
@@ -460,6 +461,13 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if key.device != dev or value.device != dev:
         raise ValueError("query, key and value must be on one device")
     scale = float(softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D))
+    inplace = out is not None and out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
+    for t in (out, lse):
+        if t is not None and (any(hxlib.overlap(t, x) for x in (key, value, query_start))
+                              or (hxlib.overlap(t, query) and not (t is out and inplace))):
+            raise ValueError("out and lse must not overlap key, value, query_start, or a part of query")
+    if out is not None and lse is not None and hxlib.overlap(out, lse):
+        raise ValueError("out and lse must not overlap")
     if out is None:
         out = query.new_empty((T, Hq, D))
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous() \

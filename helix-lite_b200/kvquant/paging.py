@@ -83,12 +83,6 @@ _I32 = torch.int32
 _SIZED = ("free_pages", "free_count", "page_refs")
 
 
-def _span(t):
-    """Addresses that a tensor reaches over: first byte, and the one past the last."""
-    lo = t.data_ptr()
-    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-
 def _row_stride(block_table):
     B, W = block_table.shape
     return int(block_table.stride(0)) if B > 1 else W
@@ -133,7 +127,7 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
         i32, i64 = free_count.new_empty, torch.int64
         out = BatchTables(i32(B + 1), i32(B), i32(T, dtype=i64), i32(T, dtype=i64), i32(1))
     else:
-        taken = [(_span(t), "one of the inputs") for t in (cached_lens, new_tokens, free_count, free_pages, block_table,
+        taken = [(hxlib.span(t), "one of the inputs") for t in (cached_lens, new_tokens, free_count, free_pages, block_table,
                                                            page_refs) if t is not None and t.numel()]
         for name, n, dt in (("query_start", B + 1, torch.int32), ("seq_lens", B, torch.int32),
                             ("slot_mapping", T, torch.int64), ("positions", T, torch.int64),
@@ -143,7 +137,7 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
             if t.shape != (n,) or t.dtype != dt or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"out.{name} must be a contiguous ({n},) {dt} tensor on {dev}")
             if n:
-                lo, hi = _span(t)
+                lo, hi = hxlib.span(t)
                 for (a, e), whose in taken:
                     if lo < e and a < hi:
                         raise ValueError(f"out.{name} must not overlap {whose}")

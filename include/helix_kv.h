@@ -472,7 +472,8 @@ HX_API int hx_prefill_attn(void* stream, const hx_pool_layer* pool, const hx_lay
  * one projection. Query head i reads KV head i / group; token i attends to
  * tokens 0 .. i of its sequence. Writes out (T, H*group, D) contiguous, in the
  * input type, and lse (T, H*group) fp32 natural log when non-NULL; rows
- * outside every sequence keep their contents. K and V of masked places are not
+ * outside every sequence keep their contents. out may be q itself (contiguous);
+ * out and lse overlap nothing else. K and V of masked places are not
  * read as numbers: infinities and NaN there change no result. softmax_scale
  * must be positive. Scores, softmax statistics and the output sum are fp32,
  * the probabilities enter the second product in the input type. One kernel.
