@@ -199,7 +199,7 @@ def prompts_into(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, at
     n = int(getattr(attn_metadata, "num_actual_tokens", query.shape[0]))
     Hq, D = query.shape[-2], query.shape[-1]
     out = output[:n].view(n, Hq, D)
-    fits = out.dtype == query.dtype and out.is_contiguous()
+    fits = out.dtype == query.dtype and out.is_contiguous() and out.data_ptr() % 16 == 0
     o, _ = fused.prompt_attention(query[:n].reshape(n, Hq, D), key[:n].reshape(n, -1, D), value[:n].reshape(n, -1, D),
                                   attn_metadata.query_start_loc, softmax_scale=scale, out=out if fits else None)
     if not fits:

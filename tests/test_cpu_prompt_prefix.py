@@ -133,3 +133,17 @@ def test_hook_attends_whole_prompts_exactly_when_asked(monkeypatch):
         assert [c[0] for c in calls] == [want]
         if want == "prompt":
             assert bool((out[:10] == 0.25).all()) and not out[10:].any()
+
+
+def test_hook_takes_an_output_off_the_kernels_alignment(monkeypatch):
+    """prompt_attention writes 16-byte pieces; any other output is copied into."""
+    bt, q, k = torch.zeros((2, 9), dtype=torch.int32), torch.randn(10, 28, 128).half(), torch.randn(10, 4, 128).half()
+    m = _meta(max_query_len=5, max_seq_len=5, num_actual_tokens=10, block_table=bt, seq_lens=torch.tensor([5, 5]),
+              query_start_loc=torch.tensor([0, 5, 10]))
+    buf = torch.zeros(12 * 28 * 128 + 8, dtype=torch.float16)
+    for shift, direct in ((0, True), (1, False), (4, False), (8, True)):
+        cb, impl, layer, calls = _hook(monkeypatch, _EXACT_PROMPTS=True, _FP16_CACHE=False)
+        out = buf.zero_()[shift:shift + 12 * 28 * 128].view(12, 28, 128)
+        impl.forward(layer, q, k, k, None, m, out)
+        assert [c[0] for c in calls] == ["prompt"] and (calls[0][2]["out"] is not None) == direct
+        assert bool((out[:10] == 0.25).all()) and not out[10:].any()
