@@ -141,6 +141,8 @@ def make_impl_cls(base):
             elif passthrough:
                 return super().forward(layer, query, key, value, kv_cache, attn_metadata, output,
                                        output_scale, output_block_scale)
+            if _EXACT_PROMPTS and not _FP16_CACHE and whole_prompts(attn_metadata, query, key):  # of one token each
+                return prompts_into(query, key, value, attn_metadata, output, scale=float(self.scale))
             return decode_into(pool, idx, query, attn_metadata, output, scale=float(self.scale))
 
     KVQuantCompactImpl.__name__ = "KVQuantCompactImpl"
@@ -184,6 +186,8 @@ def whole_prompts(attn_metadata, query: torch.Tensor, key: torch.Tensor) -> bool
     """Whether every sequence of the batch is a whole prompt, as far as the
     host can tell without reading the device: all chunks of the longest
     chunk's length, and no sequence longer than that."""
+    if getattr(attn_metadata, "query_start_loc", None) is None:
+        return False
     n = int(getattr(attn_metadata, "num_actual_tokens", query.shape[0]))
     B = int(attn_metadata.query_start_loc.shape[0]) - 1
     longest = int(attn_metadata.max_query_len)

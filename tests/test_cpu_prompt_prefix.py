@@ -147,3 +147,17 @@ def test_hook_takes_an_output_off_the_kernels_alignment(monkeypatch):
         impl.forward(layer, q, k, k, None, m, out)
         assert [c[0] for c in calls] == ["prompt"] and (calls[0][2]["out"] is not None) == direct
         assert bool((out[:10] == 0.25).all()) and not out[10:].any()
+
+
+def test_hook_attends_one_token_prompts_exactly_too(monkeypatch):
+    """A batch of one-token prompts is a batch of whole prompts; one-token steps
+    of longer sequences, or without the option, decode from the pool."""
+    bt, q, k = torch.zeros((3, 9), dtype=torch.int32), torch.randn(3, 28, 128).half(), torch.randn(3, 4, 128).half()
+    for asked, cache, longest, want in ((True, False, 1, "prompt"), (True, False, 2, "decode"), (False, False, 1, "decode"),
+                                        (True, True, 1, "decode")):
+        cb, impl, layer, calls = _hook(monkeypatch, _EXACT_PROMPTS=asked, _FP16_CACHE=cache)
+        out = torch.zeros(3, 28, 128, dtype=torch.float16)
+        m = _meta(max_query_len=1, max_seq_len=longest, num_actual_tokens=3, block_table=bt,
+                  seq_lens=torch.full((3,), longest), query_start_loc=torch.tensor([0, 1, 2, 3]))
+        impl.forward(layer, q, k, k, None, m, out)
+        assert [c[0] for c in calls] == [want]
