@@ -34,8 +34,9 @@ kernels flag any block id past it.
 
 Two options, off by default: ``shared_prefix=True`` lets a decode batch that
 attends to every block (``top_k_blocks_decode=0``) and whose metadata names a
-common prefix (vLLM's ``common_prefix_len``) read that prefix once for the
-whole batch (fused.shared_prefix_decode); ``exact_prompts=True`` lets a batch of
+common prefix (vLLM's ``common_prefix_len``) that outweighs the sequences' own
+tokens (``shares_prefix``) read that prefix once (fused.shared_prefix_decode,
+whose probabilities are fp16); ``exact_prompts=True`` lets a batch of
 whole prompts, without the fp16 cache, attend to its own K and V before their
 quantisation (fused.prompt_attention) instead of reading them back from the pool.
 
@@ -166,7 +167,7 @@ def decode_into(pool: CompactKVPool, idx: int, query: torch.Tensor, attn_metadat
     if _TOP_K > 0:
         sel = fused.quest_select(pool, idx, q, bt, seq_lens, top_k=_TOP_K, sink_pages=_SINK_BLOCKS, gqa=_GQA)
         o, _ = fused.decode(pool, idx, q, bt, seq_lens, sel, softmax_scale=scale, v_pos="physical")
-    elif _SHARED_PREFIX and B > 1 and common_prefix(attn_metadata, pool.block_size) > 0:
+    elif _SHARED_PREFIX and shares_prefix(pool, B, attn_metadata):
         o, _ = fused.shared_prefix_decode(pool, idx, q, bt, seq_lens, common_prefix(attn_metadata, pool.block_size),
                                           softmax_scale=scale, v_pos="physical")
     else:
@@ -180,6 +181,27 @@ def common_prefix(attn_metadata, block_size: int) -> int:
     """Tokens in whole blocks that every sequence of the batch shares, as vLLM's
     metadata says (0 where it says nothing)."""
     return int(getattr(attn_metadata, "common_prefix_len", 0) or 0) // block_size * block_size
+
+
+def shares_prefix(pool: CompactKVPool, B: int, attn_metadata) -> bool:
+    """Whether a decode batch is better served by reading its common prefix
+    once. shared_prefix_decode saves (B - 1) readings of the prefix, at about 0.1 ns a
+    token and KV head, but leaves a sequence's own tokens to one CTA a head, at
+    12.8 ns a token, where fused.decode spreads them over the SMs; 64 * own <=
+    heads * (B - 1) * prefix weighs the two. Over 2,040 batches (1 to 8 KV heads,
+    2 to 64 sequences, prefixes of 128 to 128K tokens, 16 to 128K own ones) that
+    is 1.4 % above the better of both in the mean. For instance, 8 sequences on
+    32K tokens take 201 us by themselves and 137 shared with 8K tokens each of
+    their own (shared is taken to 14K), 321 and 481 with 32K; on 2K, 35 and 21
+    with 512, 70 and 118 with 8K. Prefixes short of a key tile gain nothing.
+    Without the longest sequence in the metadata the option decides alone."""
+    common = common_prefix(attn_metadata, pool.block_size)
+    if B < 2 or common == 0:
+        return False
+    longest = int(getattr(attn_metadata, "max_seq_len", 0) or 0)
+    if longest == 0:
+        return True
+    return common >= 128 and 64 * max(0, longest - common) <= pool.num_kv_heads * (B - 1) * common
 
 
 def whole_prompts(attn_metadata, query: torch.Tensor, key: torch.Tensor) -> bool:

@@ -161,3 +161,21 @@ def test_hook_attends_one_token_prompts_exactly_too(monkeypatch):
                   seq_lens=torch.full((3,), longest), query_start_loc=torch.tensor([0, 1, 2, 3]))
         impl.forward(layer, q, k, k, None, m, out)
         assert [c[0] for c in calls] == [want]
+
+
+def test_hook_reads_a_shared_prefix_once_only_where_that_pays(monkeypatch):
+    """A short common prefix before long sequences of their own goes to the
+    per-sequence decode, which splits every sequence over the SMs."""
+    bt, q = torch.zeros((64, 9), dtype=torch.int32), torch.randn(64, 28, 128)
+    for B, H, common, longest, want in (
+            (4, 4, 2048, 2048 + 300, "shared"), (4, 4, 2048, 2048 + 400, "decode"),       # 64 own <= H (B - 1) common
+            (8, 4, 2048, 2048 + 32768, "decode"), (2, 4, 4096, 4096 + 131072, "decode"),
+            (64, 4, 32768, 32768 + 512, "shared"), (64, 8, 2048, 2048 + 16000, "shared"), (8, 1, 2048, 2048 + 512, "decode"),
+            (64, 4, 112, 112, "decode"), (64, 4, 128, 130, "shared"), (3, 4, 1024, 0, "shared")):  # no length known
+        cb, impl, layer, calls = _hook(monkeypatch, _SHARED_PREFIX=True)
+        cb._POOL.num_kv_heads = H
+        out = torch.zeros(64, 28, 128, dtype=torch.float16)
+        impl.forward(layer, q, None, None, None, _meta(max_query_len=1, num_actual_tokens=B, block_table=bt,
+                                                       seq_lens=torch.full((64,), longest), common_prefix_len=common,
+                                                       max_seq_len=longest), out)
+        assert [c[0] for c in calls] == [want], (B, H, common, longest)
