@@ -54,6 +54,7 @@ struct Smem {
   float2 ml[ROWS];                               // the second stream's (maximum, sum) of each row
   uint64_t q_full[2], kv_full[STAGES], kv_empty[STAGES], s_full[2], p_full[2], o_full[2], ml_full, ml_empty, drain;
   uint32_t tmem, abort;
+  int row;                                       // the prefix's table row
 };
 
 struct Params {
@@ -87,7 +88,8 @@ struct Item {
   bool two, suffix;                         // two query tiles (else one tile, two streams of key tiles)
 };
 
-HX_DEVINL bool get_item(const Params& p, int j, int idx, Item& it) {
+// row: the table row that the prefix is read from, -1 if no sequence holds the prefix.
+HX_DEVINL bool get_item(const Params& p, int j, int row, int idx, Item& it) {
   const int pre = p.RB * p.n_splits, lead = j < pre ? 1 : 0;
   if (idx < lead) {
     const int rb = j % p.RB, split = j / p.RB;
@@ -97,10 +99,10 @@ HX_DEVINL bool get_item(const Params& p, int j, int idx, Item& it) {
     const int nt = (p.prefix_pages + PAGES - 1) / PAGES;
     const int ta = (int)((int64_t)nt * split / p.n_splits), te = (int)((int64_t)nt * (split + 1) / p.n_splits);
     it.page0 = ta * PAGES;
-    it.pages = min(te * PAGES, p.prefix_pages) - it.page0;
+    it.pages = row < 0 ? 0 : min(te * PAGES, p.prefix_pages) - it.page0;
     it.tokens = it.pages * S;
     it.pidx = split;
-    it.trow = 0;
+    it.trow = (int64_t)row * p.bt_stride;
   } else {
     const int first = j - pre % p.J;
     const int b = (first < 0 ? first + p.J : first) + (idx - lead) * p.J;
@@ -180,7 +182,7 @@ HX_DEVINL void produce(const Params& p, Smem& sm, int h, int j, int w) {
   constexpr int kNone = -0x7fffffff;  // past the item's pages
   int g = 0;                          // tiles so far: stage 2 (g & 1) + KV
   Item it;
-  for (int idx = 0; get_item(p, j, idx, it); ++idx) {
+  for (int idx = 0; get_item(p, j, sm.row, idx, it); ++idx) {
     const int32_t* bt = p.bt + it.trow + it.page0 + w;
     const int pages = it.pages - w;
     auto entry = [&](int i) -> int { return PAGES * i < pages ? bt[PAGES * i] : kNone; };
@@ -354,6 +356,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
     }
     __syncwarp();
     tc::tmem_alloc(&sm.tmem, 512);
+    // ---- the first row that is neither padding nor too short names the prefix's pages
+    const int64_t least = max((int64_t)p.prefix_pages * S, (int64_t)1);
+    int row = -1;
+    for (int b0 = 0; b0 < p.B && row < 0; b0 += 32) {
+      const uint32_t m = __ballot_sync(0xffffffffu, b0 + lane < p.B && p.seq_lens[b0 + lane] >= least);
+      if (m) row = b0 + __ffs(m) - 1;
+    }
+    if (lane == 0) sm.row = row;
   }
   // ---- level tables of the head
   auto kpole = [&](int d, int c) -> uint32_t {
@@ -393,7 +403,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
     const uint32_t sb = tmem + lanes + 128 * q, ob = tmem + lanes + 256 + 128 * q;
     int used = 0, done = 0, joined = 0;  // S tiles, O results and joined items of this warpgroup so far
     bool ok = true;
-    for (int idx = 0; ok && get_item(p, j, idx, it); ++idx) {
+    for (int idx = 0; ok && get_item(p, j, sm.row, idx, it); ++idx) {
       const int seq = it.seq0 + (it.two ? q * TQ : 0) + r / G;
       const bool live = it.suffix ? r < G : (r < TQ * G && seq < p.B);
       const bool any = __any_sync(0xffffffffu, live);  // warps without rows only keep step
@@ -571,10 +581,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
     bool ok = true;
     int g = 0, buf = 0;  // tiles so far; the query buffer of the next one-tile item
     bool ahead = false;  // its rows are on the way
-    bool more = get_item(p, j, 0, it);
+    bool more = get_item(p, j, sm.row, 0, it);
     for (int idx = 0; ok && more; ++idx) {
       const Item now = it;
-      more = get_item(p, j, idx + 1, it);
+      more = get_item(p, j, sm.row, idx + 1, it);
       if (now.n == 0) continue;
       if (now.two) {
         load_q(0, now.seq0);

@@ -352,7 +352,8 @@ def shared_prefix_decode(pool: CompactKVPool, layer_idx: int, query: torch.Tenso
 
     query (B, Hq, 128) fp16, one token per sequence; block_table (B, max_pages)
     and seq_lens (B,) as for ``decode``, with the first prefix_len / 16 entries
-    of every row naming the same pool pages (read from row 0). ``prefix_len`` is
+    of every row naming the same pool pages (read from the first row with
+    tokens). ``prefix_len`` is
     a host number of tokens, a multiple of the page size. The prefix's pages
     are read and dequantised once for up to 2 * floor(128 / group) sequences
     (again for each further block of so many) and meet all their query rows in

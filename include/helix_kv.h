@@ -491,9 +491,10 @@ HX_API int hx_prompt_attn(void* stream, int32_t dtype, const void* q, int64_t q_
  * prefix_pages pool pages: the prefix is read and dequantised once for all of
  * them. q (B, H*group, D) fp16 contiguous (group <= 128, D = 128, page size 16);
  * block_table (B rows of bt_stride entries) holds each sequence's whole table,
- * of which the first prefix_pages entries are read from row 0 only; seq_lens[b]
- * counts all tokens and is at least 16 * prefix_pages, or 0 for a padding row
- * (out 0, lse -inf); a shorter one is HX_DEV_ERR_BOUNDS and its row as for
+ * of which the first prefix_pages entries are read from the first row with
+ * tokens only; seq_lens[b] counts all tokens and is at least 16 * prefix_pages,
+ * or 0 for a padding row (out 0, lse -inf; its table row is not read); a shorter
+ * one is HX_DEV_ERR_BOUNDS and its row as for
  * padding. All pages are attended (no selection). V rows by the logical
  * position, or the physical one with HX_VPOS_PHYSICAL in flags. n_splits: CTAs
  * along the prefix per (KV head, block of query rows), hx_prefix_splits() or any
