@@ -1,5 +1,6 @@
 // Decode attention of a batch whose sequences share a long prefix of pool
-// pages: the prefix is read and dequantised once for the whole batch.
+// pages: the prefix is read and dequantised once for each block of query rows
+// (two tiles of 128: 36 sequences at a group of 7), not for every sequence.
 //
 //   o_b = softmax over the sequence's tokens of (scale q_b . k_j) v_j,  the
 //   first prefix_len tokens being the same pool pages for every sequence
@@ -25,11 +26,13 @@
 //   24     the query tiles and the matrix products (tcgen05.mma, one thread)
 //
 // What bounds it: at 8 sequences behind 1M tokens (nuq4, 409 us, 1.46 TB/s of
-// codes; fused.decode, which reads the prefix per sequence: 4,967) the
-// shared-memory pipe (59 % for table lookups, operand stores and waits, 24 %
-// more for the tensor core's operands) and issue slots (55 %) of 16
-// dequantising warps. At 64 sequences behind 32K (84 us) the softmax's two
-// passes and the 64 suffixes.
+// codes, outlier lists and their records; fused.decode, which reads the prefix
+// per sequence: 4,964) the shared-memory pipe (59 % for table lookups, operand
+// stores and waits, 24 % more for the tensor core's operands) and issue slots
+// (55 %) of 16 dequantising warps. At 64 sequences behind 32K (84 us) the softmax's two
+// passes and the 64 suffixes. A suffix is one item, whatever its length: 1.6 us
+// a key tile, so sequences much longer than the prefix are better served by
+// fused.decode, which splits them.
 #include "dequant.cuh"
 #include "tcgen.cuh"
 #include "tmap.cuh"
@@ -668,7 +671,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) prefix_kernel(const __grid_consta
 }
 
 // Joins a row's partials: weights 2^(m - M), M the largest m; one CTA a row,
-// its warps take every fourth partial.
+// its warps take the partials in turns of 32 (37 splits and a suffix: two warps).
 constexpr int MW = 4;
 struct MergeParams {
   const float* part_o;

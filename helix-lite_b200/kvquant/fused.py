@@ -12,7 +12,7 @@ fp16 staging buffer (src/kvquant/compact_backend.py:225-299):
                  normalised o (fp32) and lse (natural log)
   selected_lists the selection as ascending page lists (API / tests)
   prefill        causal attention of prompt chunks, read from the pool
-  shared_prefix_decode  decode of a batch on one prefix, read once for all
+  shared_prefix_decode  decode of a batch on one prefix, read once for many
   prompt_attention  causal attention of whole prompts from their own K and V
 
 quest_select also returns, per (b, h), how many pages each slice of the

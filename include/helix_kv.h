@@ -488,8 +488,9 @@ HX_API int hx_prompt_attn(void* stream, int32_t dtype, const void* q, int64_t q_
 
 /*
  * One decode token per sequence of a batch whose sequences share their first
- * prefix_pages pool pages: the prefix is read and dequantised once for all of
- * them. q (B, H*group, D) fp16 contiguous (group <= 128, D = 128, page size 16);
+ * prefix_pages pool pages: the prefix is read and dequantised once for each
+ * 2 floor(128 / group) of them. A sequence's further pages are read by one CTA a
+ * KV head. q (B, H*group, D) fp16 contiguous (group <= 128, D = 128, page size 16);
  * block_table (B rows of bt_stride entries) holds each sequence's whole table,
  * of which the first prefix_pages entries are read from the first row with
  * tokens only; seq_lens[b] counts all tokens and is at least 16 * prefix_pages,
