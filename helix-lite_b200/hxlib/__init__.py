@@ -225,7 +225,16 @@ def err_word(device) -> torch.Tensor:
     key = dev.index if dev.index is not None else torch.cuda.current_device()
     w = _err_words.get(key)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+        d = torch.device("cuda", key)
+        with torch.cuda.device(d):
+            if torch.cuda.is_current_stream_capturing():
+                # cleared on a stream outside the capture: as part of the graph, each replay would clear it again and
+                # lose what was flagged since the last
+                w = torch.empty(1, dtype=torch.int32, device=d)
+                with torch.cuda.stream(torch.cuda.Stream(d)):
+                    w.zero_()
+            else:
+                w = torch.zeros(1, dtype=torch.int32, device=d)
         _err_words[key] = w
     return w
 
