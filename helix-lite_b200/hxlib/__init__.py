@@ -212,6 +212,7 @@ def require_cuda(*tensors):
 
 _err_words: dict = {}
 _scratch: dict = {}
+_outgrown: list = []
 
 
 def err_ptr(index: int) -> int:
@@ -256,13 +257,19 @@ def scratch(device, name: str, nbytes: int) -> torch.Tensor:
     """Grow-only, zero-initialised byte buffer per (device, name).
 
     Kernels that count into scratch leave it zero on exit, so a buffer is
-    zeroed once at allocation only.
+    zeroed once at allocation only. A buffer that has become too small is kept
+    for good: captured graphs go on writing into it. Sizes at least double, so
+    what is kept is at most the size in use.
     """
     dev = torch.device(device)
     key = (dev.index if dev.index is not None else torch.cuda.current_device(), name)
     buf = _scratch.get(key)
     if buf is None or buf.numel() < nbytes:
-        buf = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=torch.device("cuda", key[0]))
+        n = max(int(nbytes), 256)
+        if buf is not None:
+            n = max(n, 2 * buf.numel())
+            _outgrown.append(buf)
+        buf = torch.zeros(n, dtype=torch.uint8, device=torch.device("cuda", key[0]))
         _scratch[key] = buf
     return buf
 

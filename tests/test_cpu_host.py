@@ -205,3 +205,26 @@ def test_slice_index_by_reciprocal_multiply_is_exact():
     for per in range(2, 16385):
         m = np.uint64(((1 << 32) + per - 1) // per)
         assert np.array_equal((x * m) >> np.uint64(32), x // np.uint64(per)), per
+
+
+def test_outgrown_scratch_stays_alive(monkeypatch):
+    """A graph captured while the scratch was smaller holds its address: the
+    buffer must not go back to the allocator, and what is kept stays bounded."""
+    import weakref
+
+    import torch
+
+    import hxlib
+    monkeypatch.setattr(hxlib, "_scratch", {})
+    monkeypatch.setattr(hxlib, "_outgrown", [], raising=False)
+    zeros = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, device=None, **kw: zeros(*a, **kw))   # no GPU here
+    seen = []
+    for n in (100, 300, 301, 1000, 1001, 5000, 10):
+        b = hxlib.scratch(torch.device("cuda", 0), "decode", n)
+        assert b.numel() >= n and not b.any()
+        seen.append((weakref.ref(b), b.data_ptr()))
+        last = b.numel()
+        del b
+    assert all(r() is not None and r().data_ptr() == p for r, p in seen)
+    assert sum(b.numel() for b in hxlib._outgrown) <= last
