@@ -114,7 +114,8 @@ def extend_tables(block_table: torch.Tensor, cached_lens: torch.Tensor, new_toke
     sequence whose new tokens would begin inside a page of more than one
     reference (a shared prefix cut to a length inside a page): its other
     holders read that page. Copy its rows to a page of the sequence's own
-    first, or cut to whole pages.
+    first (CompactKVPool.unpack_to_staging, then write_kv), or cut to whole
+    pages.
     """
     n_pages = _check(block_table, page_size, num_pages, free_pages, free_count, page_refs, cached_lens=cached_lens,
                      new_tokens=new_tokens)

@@ -237,3 +237,55 @@ def test_outputs_that_alias_are_refused():
     ok = paging.extend_tables(table, cached, new, free, count, num_tokens=3, page_refs=refs,
                               out=out(slot_mapping=torch.cat([long, long])[:3], query_start=_i32([0, 0, 0, 0])[1:3]))
     assert ok.slot_mapping.tolist() == [32, 33, 34] and ok.seq_lens.tolist() == [3]
+
+
+def test_a_shared_page_is_copied_by_hand_and_extended():
+    """What the refusal asks for: the page's rows read back and written to a page
+    of the sequence's own (levels and outliers quantise to themselves), then
+    both sequences go on, each as if it had never shared."""
+    from kvquant import paging
+    from kvquant.compact_pool import CompactKVPool
+    from kvquant.synthetic import NUQ4, make_kv, make_scales
+    import hxlib
+    H, D, S, NB = 2, 128, 16, 16
+    sc = make_scales([NUQ4], H, D, t_cal=128, seed=5)
+    pool, alone = CompactKVPool(1, NB, S, H, D, sc), CompactKVPool(1, NB, S, H, D, sc)
+    K, V = make_kv(64, H, D, seed=6, chan_seed=5, outlier_frac=0.05)
+    table = torch.full((2, 6), -1, dtype=torch.int32, device="cuda")
+    free, refs, count = _i32(np.arange(NB)), torch.zeros(NB, dtype=torch.int32, device="cuda"), _i32([NB])
+    t = paging.extend_tables(table[:1], _i32([0]), _i32([40]), free, count, num_tokens=40, page_refs=refs)
+    pool.write_kv(0, K[:40], V[:40], t.slot_mapping, t.positions)
+    table[1] = table[0]
+    refs[table[0, :3].long()] += 1
+    lens, count = paging.truncate_tables(table, _i32([40, 40]), _i32([40, 37]), free, t.free_count, page_refs=refs)
+    assert lens.tolist() == [40, 37] and int(count) == NB - 3
+    new = _i32([2, 3])
+    paging.extend_tables(table, lens, new, free, count, num_tokens=5, page_refs=refs)
+    _flagged("shared page")
+    # sequence 1 takes a page of its own in place of the third, with the 5 tokens it keeps there
+    old = table[1, 2].clone()
+    sk, sv = (torch.empty((1, S, H, D), dtype=torch.float16, device="cuda") for _ in range(2))
+    pool.unpack_to_staging(0, old[None], torch.tensor([32], device="cuda"), sk, sv)
+    own = free[count.long() - 1]
+    count -= 1
+    at = torch.arange(5, device="cuda")
+    pool.write_kv(0, sk[0, :5].contiguous(), sv[0, :5].contiguous(), own.long() * S + at, 32 + at)
+    table[1, 2] = own[0]
+    refs[old.long()] -= 1
+    refs[own.long()] += 1
+    t = paging.extend_tables(table, lens, new, free, count, num_tokens=5, page_refs=refs)
+    hxlib.check_device_errors()
+    # sequence 0 goes on with tokens 40, 41, sequence 1 with 50 .. 52
+    pool.write_kv(0, K[[40, 41, 50, 51, 52]].contiguous(), V[[40, 41, 50, 51, 52]].contiguous(), t.slot_mapping, t.positions)
+    for b, toks in ((0, list(range(42))), (1, list(range(37)) + [50, 51, 52])):
+        n = len(toks)
+        i = torch.arange(n, device="cuda")
+        alone.reset_pages(0, torch.arange(3, dtype=torch.int32, device="cuda"))
+        alone.write_kv(0, K[toks].contiguous(), V[toks].contiguous(), i, i)
+        got, want = [], []
+        for p, pages, out in ((pool, table[b, :3], got), (alone, torch.arange(3, device="cuda"), want)):
+            k, v = (torch.empty((3, S, H, D), dtype=torch.float16, device="cuda") for _ in range(2))
+            p.unpack_to_staging(0, pages, torch.arange(3, device="cuda") * S, k, v)
+            p.check()
+            out += [k.view(-1, H, D)[:n], v.view(-1, H, D)[:n]]
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
